@@ -17,7 +17,12 @@ EXT       := $(shell $(PYTHON) -c "import sysconfig;print(sysconfig.get_config_v
 
 OPT       ?= -O3
 INC       := -Icsrc/include -Icsrc/kernels
-HIPFLAGS  := --offload-arch=$(ARCH) $(OPT) -std=c++20 -fPIC $(INC) -Wall -Wno-unused-result
+# no packed fp32 instructions (v_pk_add/mul/fma_f32): the compiler forms them
+# from ordinary float code at -O3, and some of their forms have given wrong
+# results now and then on these GPUs.  (The host pass does not know the
+# feature and says so; that is harmless.)
+NOPK      := -Xclang -target-feature -Xclang -packed-fp32-ops
+HIPFLAGS  := --offload-arch=$(ARCH) $(OPT) -std=c++20 -fPIC $(INC) -Wall -Wno-unused-result $(NOPK)
 CXXFLAGS  := $(OPT) -std=c++17 -fPIC $(INC) -Wall -Wno-unused-result
 HOSTHIP   := -D__HIP_PLATFORM_AMD__ -I$(ROCM)/include
 LDHIP     := -L$(ROCM)/lib -lamdhip64 -Wl,-rpath,$(ROCM)/lib

@@ -115,7 +115,9 @@ __device__ __forceinline__ void d_index(const Conv1DirectParams& p, int* sidx, i
   if ((int)threadIdx.x < nimg) sidx[threadIdx.x] = p.idx ? p.idx[img0 + threadIdx.x] : img0 + threadIdx.x;
 }
 
-// fp32 pairs: one v_pk_fma_f32 does two FMAs (the VALU's full fp32 rate).
+// fp32 pairs, written for v_pk_fma_f32 (two FMAs, the VALU's full fp32 rate).
+// The build turns packed fp32 instructions off (Makefile, NOPK), so a pair is
+// two v_fma_f32 today; the layout below is the same either way.
 // Accumulators pair adjacent channels; the other operand is one input value
 // splatted to both halves.  Input values are kept as register PAIRS (f2) and
 // splatted with a shuffle that folds into the instruction's op_sel: a lone

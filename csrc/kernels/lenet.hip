@@ -646,8 +646,8 @@ __global__ void __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(4))) le
         const int key = max3i(max3i(k0, k1, k2), k3, 0);
         a1s[ea1 + tile_c(T)] = (uint8_t)(key > 3 ? (~key & 3) : 4);
         // the two code bits left in the value perturb it by < 2^-21: below the
-        // bf16 rounding.  Scale and convert two tiles at a time (v_pk_mul_f32,
-        // one v_cvt_pk_bf16_f32)
+        // bf16 rounding.  Scale and convert two tiles at a time (one
+        // v_cvt_pk_bf16_f32)
         if (T & 1) {
           typedef float f2 __attribute__((ext_vector_type(2)));
           typedef bf16 b2 __attribute__((ext_vector_type(2)));

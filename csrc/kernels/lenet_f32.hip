@@ -15,8 +15,10 @@
 // which conv_direct_dw / conv1_direct_dw_w3 (conv_direct.hip) evaluate with
 // three zero gradients per window.  The argmax moves the patch per
 // (channel, window), so the gather is not a GEMM: these run on the VALU
-// (v_pk_fma_f32, the full fp32 rate -- gfx950's fp32 matrix rate is the same,
-// and an MFMA form would have to do the dense 4x work).
+// (packed pairs; as v_pk_fma_f32 the full fp32 rate, which is gfx950's fp32
+// matrix rate -- an MFMA form would have to do the dense 4x work.  The build
+// turns packed fp32 instructions off (Makefile, NOPK): a pair is two
+// v_fma_f32).
 //
 //  * conv2 dW: a lane owns one output channel co (16 per wave row) and one
 //    window slot; its 6 input channels x 25 taps of accumulators are 75
