@@ -10,6 +10,7 @@
 
 #include <hip/hip_runtime_api.h>
 
+#include "feedforward.h"
 #include "kernels.h"
 #include "mcc/cpu_net.h"
 #include "mcc/engine.h"
@@ -653,6 +654,38 @@ PYBIND11_MODULE(_C, m) {
   k.attr("EPI_LOGITS") = (int)gpu::EPI_LOGITS;
   k.attr("EPI_DACT") = (int)gpu::EPI_DACT;
   k.attr("EPI_PARTIAL") = (int)gpu::EPI_PARTIAL;
+  // ---- feed-forward / 8-bit / distillation operators (feedforward.h) ----
+  k.def("gated_forward",
+        [](int M, int D, int F, int act, uintptr_t x, int64_t ldx, uintptr_t wg, uintptr_t wu, int64_t ldw, uintptr_t h,
+           uintptr_t gate, uintptr_t up, uintptr_t s) {
+          gpu::GatedParams p;
+          p.M = M; p.D = D; p.F = F; p.act = act;
+          p.x = ptr<void>(x); p.ldx = ldx;
+          p.wg = ptr<void>(wg); p.wu = ptr<void>(wu); p.ldw = ldw;
+          p.h = ptr<void>(h); p.gate = ptr<void>(gate); p.up = ptr<void>(up);
+          gpu::gated_forward(p, stream_of(s));
+        },
+        py::arg("M"), py::arg("D"), py::arg("F"), py::arg("act"), py::arg("x"), py::arg("ldx"), py::arg("wg"),
+        py::arg("wu"), py::arg("ldw"), py::arg("h"), py::arg("gate") = 0, py::arg("up") = 0, py::arg("stream") = 0);
+  k.def("linear_i8",
+        [](int M, int N, int K, int act, uintptr_t x, int64_t ldx, uintptr_t sx, uintptr_t w, int64_t ldw, uintptr_t sw,
+           uintptr_t bias, uintptr_t y, bool f32, uintptr_t s) {
+          gpu::LinearI8Params p;
+          p.M = M; p.N = N; p.K = K; p.act = act;
+          p.x = ptr<void>(x); p.ldx = ldx; p.sx = ptr<float>(sx);
+          p.w = ptr<void>(w); p.ldw = ldw; p.sw = ptr<float>(sw);
+          p.bias = ptr<float>(bias); p.y = ptr<void>(y); p.f32 = f32;
+          gpu::linear_i8(p, stream_of(s));
+        },
+        py::arg("M"), py::arg("N"), py::arg("K"), py::arg("act"), py::arg("x"), py::arg("ldx"), py::arg("sx"),
+        py::arg("w"), py::arg("ldw"), py::arg("sw"), py::arg("bias"), py::arg("y"), py::arg("f32"),
+        py::arg("stream") = 0);
+  k.attr("GATE_NONE") = (int)gpu::GATE_NONE;
+  k.attr("GATE_RELU") = (int)gpu::GATE_RELU;
+  k.attr("GATE_TANH") = (int)gpu::GATE_TANH;
+  k.attr("GATE_SILU") = (int)gpu::GATE_SILU;
+  k.attr("GATE_GELU") = (int)gpu::GATE_GELU;
+  k.attr("LINEAR_I8_MAX_K") = gpu::kLinearI8MaxK;
   k.attr("ACT_NONE") = (int)gpu::ACT_NONE;
   k.attr("ACT_RELU") = (int)gpu::ACT_RELU;
   k.attr("ACT_TANH") = (int)gpu::ACT_TANH;

@@ -1,0 +1,175 @@
+// Gated feed-forward block, bf16:
+//
+//   G = X Wg^T, U = X Wu^T, H = f(G) * U          f: none, relu, tanh, silu, gelu
+//
+// Forward: one launch.  A tile multiplies the same X rows with the matching
+// rows of both weights (tile_gemm.h, SPLIT), so a lane ends with G and U of the
+// same outputs and the activation, the product and the rounding happen on the
+// accumulators: H is rounded once from 32-bit sums, as are the G and U that a
+// training step keeps.
+#include "feedforward.h"
+#include "few_rows.h"
+#include "kernels.h"
+#include "mcc/common.h"
+#include "tile_gemm.h"
+
+namespace mcc {
+namespace gpu {
+
+namespace {
+
+using tile::Bf16;
+using tile::FewRows;
+using tile::Operands;
+using tile::Tile;
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int A> __device__ __forceinline__ float gate_f(float v) {
+  if constexpr (A == GATE_RELU) return v > 0.f ? v : 0.f * v;  // keeps a NaN
+  if constexpr (A == GATE_TANH) return tanhf(v);
+  if constexpr (A == GATE_SILU) return v / (1.f + __builtin_amdgcn_exp2f(-kLog2e * v));
+  if constexpr (A == GATE_GELU) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+  return v;
+}
+
+// calls f with the activation as a compile-time constant
+template <class Fn> __host__ __device__ __forceinline__ void with_gate(int act, Fn&& f) {
+  switch (act) {
+    case GATE_RELU: f(ActK<GATE_RELU>{}); break;
+    case GATE_TANH: f(ActK<GATE_TANH>{}); break;
+    case GATE_SILU: f(ActK<GATE_SILU>{}); break;
+    case GATE_GELU: f(ActK<GATE_GELU>{}); break;
+    default: f(ActK<GATE_NONE>{}); break;
+  }
+}
+
+// 16 consecutive outputs of one row from column n on: two stores where the
+// row's pitch keeps 16-byte alignment (`wide`) and all of them exist
+__device__ __forceinline__ void put16(bf16* out, int64_t at, int n, int N, bool wide, const float (&v)[16]) {
+#pragma unroll
+  for (int k = 0; k < 16; k += 8) {
+    if (wide && n + k + 8 <= N) {
+      const bf16x4 a = cvt4(v[k], v[k + 1], v[k + 2], v[k + 3]), b = cvt4(v[k + 4], v[k + 5], v[k + 6], v[k + 7]);
+      store8(out + at + k, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+#pragma unroll
+      for (int e = k; e < k + 8; ++e)
+        if (n + e < N) out[at + e] = (bf16)v[e];
+    }
+  }
+}
+
+Operands operands(const GatedParams& p) {
+  Operands o;
+  o.a[0] = static_cast<const char*>(p.wg);
+  o.a[1] = static_cast<const char*>(p.wu);
+  o.b = static_cast<const char*>(p.x);
+  o.lda = p.ldw * 2;
+  o.ldb = p.ldx * 2;
+  o.arows = p.F;
+  o.brows = p.M;
+  o.kbytes = round_up(p.D, 8) * 2;
+  return o;
+}
+
+template <int FA, int FB, int KS, int NST, int WPE, int ACT>
+__global__ void __launch_bounds__(tile::kThreads, WPE) gated_tile_kernel(GatedParams p, Operands op) {
+  typedef Tile<Bf16, FA, FB, KS, NST, true> T;
+  __shared__ __attribute__((aligned(128))) char lds[T::kLds];
+  int ta, tb;
+  tile::tile_of(cdiv(p.F, T::RA / 2), cdiv(p.M, T::RB), ta, tb);
+  const int f0 = ta * (T::RA / 2), m0 = tb * T::RB;
+  T t;
+  t.run(op, lds, f0, m0, 0, (int)((op.kbytes + KS - 1) / KS));
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r32 = lane & 31, g = lane >> 5, wa = wave >> 1, wb = wave & 1;
+  const int M = p.M, F = p.F;
+  const bool wide = F % 8 == 0;
+  bf16* h = static_cast<bf16*>(p.h);
+  bf16* gate = static_cast<bf16*>(p.gate);
+  bf16* up = static_cast<bf16*>(p.up);
+#pragma unroll
+  for (int i = 0; i < FA / 2; ++i) {
+    const int f = f0 + T::a_out(wa, i, g);
+#pragma unroll
+    for (int j = 0; j < FB; ++j) {
+      const int m = m0 + T::b_out(wb, j, r32);
+      if (m >= M || f >= F) continue;
+      float gv[16], uv[16], hv[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        gv[e] = t.acc[i][j][e];
+        uv[e] = t.acc[FA / 2 + i][j][e];
+        hv[e] = gate_f<ACT>(gv[e]) * uv[e];
+      }
+      const int64_t at = (int64_t)m * F + f;
+      put16(h, at, f, F, wide, hv);
+      if (gate) {
+        put16(gate, at, f, F, wide, gv);
+        put16(up, at, f, F, wide, uv);
+      }
+    }
+  }
+}
+
+template <int FB, int U, int NW>
+__global__ void __launch_bounds__(64 * NW) gated_rows_kernel(GatedParams p, Operands op) {
+  typedef FewRows<Bf16, FB, U, NW, 2> R;
+  __shared__ __attribute__((aligned(16))) char lds[R::kLds];
+  const int f0 = blockIdx.x * 16, m0 = blockIdx.y * R::kRows;
+  R::run(op, lds, f0, m0);
+  bf16* h = static_cast<bf16*>(p.h);
+  bf16* gate = static_cast<bf16*>(p.gate);
+  bf16* up = static_cast<bf16*>(p.up);
+  with_gate(p.act, [&](auto k) {
+    for (int i = threadIdx.x; i < R::kRows * 16; i += 64 * NW) {
+      const int f = f0 + (i & 15), m = m0 + (i >> 4);
+      if (f >= p.F || m >= p.M) continue;
+      const float gv = R::template sum<float>(lds, 0, i >> 4, i & 15);
+      const float uv = R::template sum<float>(lds, 1, i >> 4, i & 15);
+      const int64_t at = (int64_t)m * p.F + f;
+      h[at] = (bf16)(gate_f<decltype(k)::v>(gv) * uv);
+      if (gate) {
+        gate[at] = (bf16)gv;
+        up[at] = (bf16)uv;
+      }
+    }
+  });
+}
+
+}  // namespace
+
+void gated_forward(const GatedParams& p, hipStream_t s) {
+  MCC_CHECK(p.M >= 0 && p.D > 0 && p.F > 0, "gated_linear: empty problem");
+  MCC_CHECK(p.act >= GATE_NONE && p.act <= GATE_GELU, "gated_linear: unknown activation");
+  MCC_CHECK(p.ldx >= round_up(p.D, 8) && p.ldw >= round_up(p.D, 8) && p.ldx % 8 == 0 && p.ldw % 8 == 0,
+            "gated_linear: row pitches must be multiples of 8");
+  MCC_CHECK(p.ldx < (1 << 22) && p.ldw < (1 << 22), "gated_linear: row pitch too large");
+  MCC_CHECK((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.wg) | reinterpret_cast<uintptr_t>(p.wu)) %
+                    16 == 0, "gated_linear: operands must be 16-byte aligned");
+  MCC_CHECK((p.gate == nullptr) == (p.up == nullptr), "gated_linear: gate and up go together");
+  if (p.M == 0) return;
+  const Operands o = operands(p);
+  if (p.M <= 64) {
+    const dim3 grid((unsigned)cdiv(p.F, 16), 1);
+    if (p.M <= 16) hipLaunchKernelGGL((gated_rows_kernel<1, 4, 4>), grid, dim3(256), 0, s, p, o);
+    else if (p.M <= 32) hipLaunchKernelGGL((gated_rows_kernel<2, 2, 4>), grid, dim3(256), 0, s, p, o);
+    else hipLaunchKernelGGL((gated_rows_kernel<4, 1, 4>), grid, dim3(256), 0, s, p, o);
+  } else if ((int64_t)cdiv(p.F, 128) * cdiv(p.M, 256) >= 256) {
+    const dim3 grid((unsigned)(cdiv(p.F, 128) * cdiv(p.M, 256)));
+    with_gate(p.act, [&](auto k) {
+      hipLaunchKernelGGL((gated_tile_kernel<4, 4, 128, 2, 1, decltype(k)::v>), grid, dim3(tile::kThreads), 0, s, p, o);
+    });
+  } else {
+    const dim3 grid((unsigned)(cdiv(p.F, 64) * cdiv(p.M, 128)));
+    with_gate(p.act, [&](auto k) {
+      hipLaunchKernelGGL((gated_tile_kernel<2, 2, 128, 2, 2, decltype(k)::v>), grid, dim3(tile::kThreads), 0, s, p, o);
+    });
+  }
+  MCC_CHECK(hipGetLastError() == hipSuccess, "gated_linear: launch failed");
+}
+
+}  // namespace gpu
+}  // namespace mcc

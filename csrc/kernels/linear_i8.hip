@@ -1,0 +1,162 @@
+// Product of 8-bit integers with a scale per token and per output channel:
+//
+//   Y[m][n] = f((sum_k Xq[m][k] Wq[n][k]) * sx[m] * sw[n] + b[n])
+//
+// The sum is exact: 32-bit integer accumulators, K bounded so that no sum of
+// products can pass them.  It becomes a 32-bit float (one rounding), is scaled
+// by the product of the two scales (two roundings), biased, and rounded to the
+// output's type.
+#include "feedforward.h"
+#include "few_rows.h"
+#include "kernels.h"
+#include "mcc/common.h"
+#include "tile_gemm.h"
+
+namespace mcc {
+namespace gpu {
+
+namespace {
+
+using tile::FewRows;
+using tile::I8;
+using tile::Operands;
+using tile::Tile;
+
+// 16 consecutive outputs of one row from column n on: 16-byte stores where the
+// row's pitch keeps their alignment (`wide`) and all of them exist
+template <class TO>
+__device__ __forceinline__ void put16(TO* out, int64_t at, int n, int N, bool wide, const float (&v)[16]) {
+#pragma unroll
+  for (int k = 0; k < 16; k += 8) {
+    if (wide && n + k + 8 <= N) {
+      if constexpr (sizeof(TO) == 2) {
+        const bf16x4 a = cvt4(v[k], v[k + 1], v[k + 2], v[k + 3]), b = cvt4(v[k + 4], v[k + 5], v[k + 6], v[k + 7]);
+        store8(out + at + k, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+      } else {
+        store8(out + at + k, f32x8{v[k], v[k + 1], v[k + 2], v[k + 3], v[k + 4], v[k + 5], v[k + 6], v[k + 7]});
+      }
+    } else {
+#pragma unroll
+      for (int e = k; e < k + 8; ++e)
+        if (n + e < N) out[at + e] = (TO)v[e];
+    }
+  }
+}
+
+// ReLU that keeps a NaN (a row whose scale is NaN stays visible)
+template <int A> __device__ __forceinline__ float act_i8(float v) {
+  if constexpr (A == ACT_RELU) return v > 0.f ? v : 0.f * v;
+  else return act_c<A>(v);
+}
+
+template <int FA, int FB, int KS, int NST, int WPE, int ACT, class TO>
+__global__ void __launch_bounds__(tile::kThreads, WPE) i8_tile_kernel(LinearI8Params p, Operands op) {
+  typedef Tile<I8, FA, FB, KS, NST, false> T;
+  __shared__ __attribute__((aligned(128))) char lds[T::kLds];
+  int ta, tb;
+  tile::tile_of(cdiv(p.N, T::RA), cdiv(p.M, T::RB), ta, tb);
+  const int n0 = ta * T::RA, m0 = tb * T::RB;
+  T t;
+  t.run(op, lds, n0, m0, 0, (int)((op.kbytes + KS - 1) / KS));
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r32 = lane & 31, g = lane >> 5, wa = wave >> 1, wb = wave & 1;
+  const int M = p.M, N = p.N;
+  const bool wide = N % 8 == 0;
+  TO* y = static_cast<TO*>(p.y);
+  float sx[FB];
+#pragma unroll
+  for (int j = 0; j < FB; ++j) sx[j] = p.sx[min(m0 + T::b_out(wb, j, r32), M - 1)];
+#pragma unroll
+  for (int i = 0; i < FA; ++i) {
+    const int n = n0 + T::a_out(wa, i, g);
+    float sw[16], b[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int c = min(n + e, N - 1);
+      sw[e] = p.sw[c];
+      b[e] = p.bias ? p.bias[c] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < FB; ++j) {
+      const int m = m0 + T::b_out(wb, j, r32);
+      if (m >= M || n >= N) continue;
+      float v[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] = act_i8<ACT>((float)t.acc[i][j][e] * (sx[j] * sw[e]) + b[e]);
+      put16(y, (int64_t)m * N + n, n, N, wide, v);
+    }
+  }
+}
+
+template <int FB, int U, int NW, class TO>
+__global__ void __launch_bounds__(64 * NW) i8_rows_kernel(LinearI8Params p, Operands op) {
+  typedef FewRows<I8, FB, U, NW, 1> R;
+  __shared__ __attribute__((aligned(16))) char lds[R::kLds];
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * R::kRows;
+  R::run(op, lds, n0, m0);
+  TO* y = static_cast<TO*>(p.y);
+  with_act(p.act, [&](auto k) {
+    for (int i = threadIdx.x; i < R::kRows * 16; i += 64 * NW) {
+      const int n = n0 + (i & 15), m = m0 + (i >> 4);
+      if (n >= p.N || m >= p.M) continue;
+      const int v = R::template sum<int>(lds, 0, i >> 4, i & 15);
+      const float b = p.bias ? p.bias[n] : 0.f;
+      y[(int64_t)m * p.N + n] = (TO)act_i8<decltype(k)::v>((float)v * (p.sx[m] * p.sw[n]) + b);
+    }
+  });
+}
+
+template <int FA, int FB, int KS, int NST, int WPE, class TO>
+void launch_tiles(const LinearI8Params& p, const Operands& o, hipStream_t s) {
+  const dim3 grid((unsigned)(cdiv(p.N, 64 * FA) * cdiv(p.M, 64 * FB)));
+  if (p.act == ACT_RELU)
+    hipLaunchKernelGGL((i8_tile_kernel<FA, FB, KS, NST, WPE, ACT_RELU, TO>), grid, dim3(tile::kThreads), 0, s, p, o);
+  else if (p.act == ACT_TANH)
+    hipLaunchKernelGGL((i8_tile_kernel<FA, FB, KS, NST, WPE, ACT_TANH, TO>), grid, dim3(tile::kThreads), 0, s, p, o);
+  else
+    hipLaunchKernelGGL((i8_tile_kernel<FA, FB, KS, NST, WPE, ACT_NONE, TO>), grid, dim3(tile::kThreads), 0, s, p, o);
+}
+
+template <class TO> void launch(const LinearI8Params& p, hipStream_t s) {
+  Operands o;
+  o.a[0] = o.a[1] = static_cast<const char*>(p.w);
+  o.b = static_cast<const char*>(p.x);
+  o.lda = p.ldw;
+  o.ldb = p.ldx;
+  o.arows = p.N;
+  o.brows = p.M;
+  o.kbytes = round_up(p.K, 16);
+  if (p.M <= 64) {
+    const dim3 grid((unsigned)cdiv(p.N, 16), 1);
+    if (p.M <= 16) hipLaunchKernelGGL((i8_rows_kernel<1, 4, 4, TO>), grid, dim3(256), 0, s, p, o);
+    else if (p.M <= 32) hipLaunchKernelGGL((i8_rows_kernel<2, 2, 4, TO>), grid, dim3(256), 0, s, p, o);
+    else hipLaunchKernelGGL((i8_rows_kernel<4, 1, 4, TO>), grid, dim3(256), 0, s, p, o);
+  } else if ((int64_t)cdiv(p.N, 256) * cdiv(p.M, 256) >= 256) {
+    launch_tiles<4, 4, 128, 2, 1, TO>(p, o, s);
+  } else if ((int64_t)cdiv(p.N, 128) * cdiv(p.M, 128) >= 256) {
+    launch_tiles<2, 2, 128, 2, 2, TO>(p, o, s);
+  } else {
+    launch_tiles<1, 1, 128, 4, 2, TO>(p, o, s);
+  }
+  MCC_CHECK(hipGetLastError() == hipSuccess, "linear_i8: launch failed");
+}
+
+}  // namespace
+
+void linear_i8(const LinearI8Params& p, hipStream_t s) {
+  MCC_CHECK(p.M >= 0 && p.N > 0 && p.K > 0, "linear_i8: empty problem");
+  MCC_CHECK(p.K <= kLinearI8MaxK, "linear_i8: K too large for an exact 32-bit sum");
+  MCC_CHECK(p.act >= ACT_NONE && p.act <= ACT_TANH, "linear_i8: unknown activation");
+  MCC_CHECK(p.ldx >= round_up(p.K, 16) && p.ldw >= round_up(p.K, 16) && p.ldx % 16 == 0 && p.ldw % 16 == 0,
+            "linear_i8: row pitches must be multiples of 16");
+  MCC_CHECK(p.ldx < (1 << 23) && p.ldw < (1 << 23), "linear_i8: row pitch too large");
+  MCC_CHECK((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w)) % 16 == 0,
+            "linear_i8: operands must be 16-byte aligned");
+  if (p.M == 0) return;
+  if (p.f32) launch<float>(p, s);
+  else launch<bf16>(p, s);
+}
+
+}  // namespace gpu
+}  // namespace mcc

@@ -1,0 +1,274 @@
+// One matrix-product tile loop for operands whose rows run along K, in units
+// of bytes so that bf16 and 8-bit integers share it:
+//
+//   C[a][b] = sum_k A[a][k] B[b][k],   A [arows][K], B [brows][K]
+//
+// A is the side that runs along the output's contiguous axis: a lane ends with
+// 16 consecutive A rows of one B row.
+//
+// The multiply is v_mfma_f32_32x32x16_bf16 or v_mfma_i32_32x32x32_i8: 32 cycles
+// each on the same fragments, lane (r, g) = (lane & 31, lane >> 5) holding 16
+// bytes of row r; a depth is 32 bytes of K, its lower half in g = 0.  A and B
+// use the same map, so any order of K inside a depth cancels.  The 32 x 32 form
+// reads half the operand registers per product of the 16 x 16 one, and its
+// accumulators stay where they are (the compiler copied 180 of 256 registers a
+// step around the 16 x 16 integer form).
+//
+// Workgroup: 4 waves in 2 x 2, wave tile (32 FA) x (32 FB), workgroup tile
+// (64 FA) x (64 FB).  Operands go HBM -> LDS by global_load_lds (16 bytes a
+// lane) into NST images of KS bytes of K; the fragments of one depth are read
+// while those of the depth before are multiplied, and the last depth of a step
+//
+//   waits for this wave's reads of image kt and its loads of step kt+1,
+//   passes the step's one barrier (now every wave has read image kt),
+//   loads step kt+NST into the place of image kt,
+//   reads depth 0 of step kt+1 and multiplies.
+//
+// At 4 x 4 fragments a wave multiplies 2048 cycles per 128 bytes of K while the
+// four waves read 128 KiB of LDS (1024 cycles at 128 B a cycle) and 64 KiB are
+// written: the matrix unit is the longer side.  Eight waves of half the tile
+// would read 192 KiB and be bound by LDS.
+//
+// An LDS row of an image is KS bytes = KS/16 slots; slot s of row r holds the
+// row's piece s ^ swz(r), applied on the source address of the load, so that
+// the 16 rows that a read phase touches fall on 16 different 16-byte bank
+// groups.  Row ρ of an A fragment is row 16 h + 4 q + e of the tile where
+// ρ = 8 q + 4 h + e: the MFMA leaves rows 8 q + 4 h + e (q, e = 0..3) of its
+// result in lane half h, which are then 16 consecutive rows.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "mfma.h"
+
+namespace mcc {
+namespace gpu {
+namespace tile {
+
+typedef __attribute__((address_space(1))) void gvoid;
+typedef __attribute__((address_space(3))) void lvoid;
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+struct Yes { static constexpr bool v = true; };
+struct No { static constexpr bool v = false; };
+
+constexpr int kThreads = 256;
+
+// what a piece behind the end of K reads
+__device__ __attribute__((aligned(64))) const uint32_t kZero16[16] = {0};
+
+struct Bf16 {
+  typedef bf16x8 frag;
+  typedef f32x4 acc;  // 16 x 16 products (few_rows.h)
+  typedef f32x16 acc32;
+  static __device__ __forceinline__ acc mul(const frag& a, const frag& b, const acc& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ acc32 mul32(const frag& a, const frag& b, const acc32& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+struct I8 {
+  typedef i32x4 frag;
+  typedef i32x4 acc;
+  typedef i32x16 acc32;
+  static __device__ __forceinline__ acc mul(const frag& a, const frag& b, const acc& c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ acc32 mul32(const frag& a, const frag& b, const acc32& c) {
+    return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
+  }
+};
+
+// a[0] / a[1]: the sources of the tile's lower and upper A half (two matrices
+// of the same shape and pitch) of a SPLIT tile, else a[0]
+struct Operands {
+  const char* a[2];
+  const char* b;
+  int64_t lda, ldb;  // row pitch in bytes (a multiple of 16, at most 2^23)
+  int arows, brows;
+  int64_t kbytes;    // bytes of K (a multiple of 16)
+};
+
+// Order of the tiles of a grid of na x nb: consecutive workgroups are dealt to
+// the 8 XCDs in turn, so workgroup i works on position (i mod 8) * n/8 + i/8 of
+// a walk over blocks of 8 B tiles: the 32 CUs of an XCD then hold about 8 x 4
+// tiles and share those 12 operand tiles in their L2.
+__device__ __forceinline__ void tile_of(int na, int nb, int& ta, int& tb) {
+  const int n = na * nb, i = (int)blockIdx.x;
+  const int q = n >> 3, r = n & 7, x = i & 7;
+  const int t = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (i >> 3);
+  constexpr int G = 8;
+  const int per = G * na;
+  const int grp = t / per, in = t - grp * per;
+  const int gb = min(G, nb - grp * G);
+  ta = in / gb;
+  tb = grp * G + (in - ta * gb);
+}
+
+template <int N> __device__ __forceinline__ void vm_wait() {
+  static_assert(N >= 0 && N < 64, "vmcnt field");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void barrier_raw() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// SPLIT: the tile's A rows are two halves of 32 FA rows from a[0] and a[1] at
+// the same place (a gate and its projection); every wave then owns FA/2
+// fragments of each.  Otherwise wave row wa owns the 32 FA rows from 32 FA wa
+// on.
+template <class E, int FA, int FB, int KS, int NST, bool SPLIT>
+struct Tile {
+  static constexpr int RA = 64 * FA, RB = 64 * FB;
+  static constexpr int kImage = (RA + RB) * KS;
+  static constexpr int kLds = NST * kImage;
+  static constexpr int kRowsPerLoad = 4096 / KS;  // rows that one load of the four waves covers
+  static constexpr int JA = RA / kRowsPerLoad, JB = RB / kRowsPerLoad;
+  static constexpr int kLoads = JA + JB;          // per thread and step
+  static constexpr int kDepths = KS / 32;
+  static constexpr int kReads = FA + FB;          // per depth
+  static constexpr int kMuls = FA * FB;
+  static_assert(KS == 128 || KS == 64, "image row");
+  static_assert(!SPLIT || (FA % 2 == 0 && JA % 2 == 0), "both halves in whole fragments and loads");
+  static_assert(kDepths % 2 == 0, "fragment buffers alternate by depth");
+  typedef typename E::frag frag;
+  typedef typename E::acc32 acc_t;
+
+  acc_t acc[FA][FB];
+
+  // first A row (within the tile; within its half when SPLIT) of the 16 that
+  // lane half h holds in fragment i
+  static __device__ __forceinline__ int a_out(int wa, int i, int h) {
+    return wa * (SPLIT ? RA / 4 : RA / 2) + 32 * (SPLIT ? i % (FA / 2) : i) + 16 * h;
+  }
+  static __device__ __forceinline__ int b_out(int wb, int j, int r) { return wb * (RB / 2) + 32 * j + r; }
+
+  // K-steps [k0, k1) of the tile whose first rows are a0 (of each half's
+  // source when SPLIT) and b0
+  __device__ __forceinline__ void run(const Operands& p, char* lds, int a0, int b0, int k0, int k1) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r32 = lane & 31, g = lane >> 5;
+    const int wa = wave >> 1, wb = wave & 1;
+    auto swz = [](int row) { return KS == 128 ? (row >> 1) & 7 : (row >> 2) & 3; };
+
+    // ---- image loads: load j of wave w covers rows from kRowsPerLoad j + (1024 / KS) w on ----
+    constexpr int kSlots = KS / 16;
+    const int lrow = wave * (1024 / KS) + lane / kSlots;
+    const int piece = ((lane % kSlots) ^ swz(lrow)) * 16;  // the same for every j: kRowsPerLoad is a period of swz
+    uint32_t va[JA], vb[JB];
+#pragma unroll
+    for (int j = 0; j < JA; ++j) {
+      const int row = j * kRowsPerLoad + lrow - (SPLIT && j >= JA / 2 ? RA / 2 : 0);
+      va[j] = (uint32_t)((int64_t)min(row, p.arows - 1 - a0) * p.lda) + piece;  // rows past the end: the last one again
+    }
+#pragma unroll
+    for (int j = 0; j < JB; ++j)
+      vb[j] = (uint32_t)((int64_t)min(j * kRowsPerLoad + lrow, p.brows - 1 - b0) * p.ldb) + piece;
+    const char* pa0 = p.a[0] + (int64_t)a0 * p.lda;
+    const char* pa1 = p.a[1] + (int64_t)a0 * p.lda;
+    const char* pb = p.b + (int64_t)b0 * p.ldb;
+    const int64_t kbytes = p.kbytes;
+
+    // load number j of step kt into the image at byte `at`; `tail`: the step may
+    // run past the end of K, where both sides read zeros
+    auto load_one = [&](int kt, int at, int j, auto tail) {
+      char* img = lds + at + wave * 1024 + j * 4096;
+      const int64_t ko = (int64_t)kt * KS;
+      const bool is_a = j < JA;
+      // (the empty asm keeps the offset a 32-bit register next to its use, so
+      // that the address is scalar base + 32-bit offset and needs no VALU)
+      uint32_t& v = is_a ? va[is_a ? j : 0] : vb[is_a ? 0 : j - JA];
+      asm volatile("" : "+v"(v));
+      const char* s = (is_a ? (SPLIT && j >= JA / 2 ? pa1 : pa0) : pb) + ko + v;
+      if (decltype(tail)::v) s = ko + piece < kbytes ? s : reinterpret_cast<const char*>(kZero16);
+      __builtin_amdgcn_global_load_lds((gvoid*)s, (lvoid*)img, 16, 0, 0);
+    };
+    auto load = [&](int kt, int at) {
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) load_one(kt, at, j, Yes{});
+    };
+
+    // ---- fragment reads: piece 2 d + g of depth d sits in slot (2 d + g) ^ swz(row) ----
+    const int rho = 16 * ((r32 >> 2) & 1) + 4 * (r32 >> 3) + (r32 & 3);
+    const int fa_at = (wa * (SPLIT ? RA / 4 : RA / 2) + rho) * KS + ((g ^ swz(rho)) << 4);
+    const int fb_at = (RA + wb * (RB / 2) + r32) * KS + ((g ^ swz(r32)) << 4);
+    frag fa[2][FA], fb[2][FB];
+    // fragment t of the FB + FA of depth d
+    auto read_one = [&](int at, int d, int t) {
+      if (t < FB) {
+        fb[d & 1][t] = *reinterpret_cast<const frag*>(lds + at + (fb_at ^ (d << 5)) + t * 32 * KS);
+      } else {
+        const int i = t - FB;
+        const int row = SPLIT ? (i >= FA / 2 ? RA / 2 : 0) + 32 * (i % (FA / 2)) : 32 * i;
+        fa[d & 1][i] = *reinterpret_cast<const frag*>(lds + at + (fa_at ^ (d << 5)) + row * KS);
+      }
+    };
+    auto mul_one = [&](int d, int q) {
+      acc[q / FB][q % FB] = E::mul32(fa[d & 1][q / FB], fb[d & 1][q % FB], acc[q / FB][q % FB]);
+    };
+
+#pragma unroll
+    for (int i = 0; i < FA; ++i)
+#pragma unroll
+      for (int j = 0; j < FB; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+
+#pragma unroll
+    for (int s = 0; s < NST; ++s)
+      if (k0 + s < k1) load(k0 + s, s * kImage);
+    if (k1 - k0 >= NST) vm_wait<(NST - 1) * kLoads>(); else vm_wait<0>();
+    barrier_raw();
+    int at = 0;  // image of step kt
+#pragma unroll
+    for (int t = 0; t < kReads; ++t) read_one(at, 0, t);
+
+    // depth d of image `at`, the reads of the next depth (of image `next`) and
+    // with `ld` the loads of step kt dealt out among its MFMAs: the source
+    // order, which the sched_barriers keep, is the schedule
+    auto depth = [&](int d, int next, auto ld, int kt) {
+#pragma unroll
+      for (int q = 0; q < kMuls; ++q) {
+        if (decltype(ld)::v) {
+#pragma unroll
+          for (int t = q * kLoads / kMuls; t < (q + 1) * kLoads / kMuls; ++t) load_one(kt, at, t, No{});
+        }
+#pragma unroll
+        for (int t = q * kReads / kMuls; t < (q + 1) * kReads / kMuls; ++t) read_one(next, (d + 1) % kDepths, t);
+        mul_one(d, q);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    auto step = [&](int kt, auto full) {
+#pragma unroll
+      for (int d = 0; d + 1 < kDepths; ++d) depth(d, at, No{}, 0);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (decltype(full)::v || kt + NST <= k1) vm_wait<(NST - 2) * kLoads>(); else vm_wait<0>();
+      barrier_raw();
+      if (!decltype(full)::v && kt + NST < k1) load(kt + NST, at);
+      const int next = at + kImage == kLds ? 0 : at + kImage;
+      depth(kDepths - 1, next, full, kt + NST);
+      at = next;
+    };
+    int kt = k0;
+    // steps whose load lies wholly inside K
+    const int kfull = min(k1, (int)(kbytes / KS)) - NST;
+    for (; kt < kfull; ++kt) step(kt, Yes{});
+    for (; kt + 1 < k1; ++kt) step(kt, No{});
+#pragma unroll
+    for (int d = 0; d + 1 < kDepths; ++d) depth(d, at, No{}, 0);
+#pragma unroll
+    for (int q = 0; q < kMuls; ++q) mul_one(kDepths - 1, q);
+  }
+};
+
+}  // namespace tile
+}  // namespace gpu
+}  // namespace mcc

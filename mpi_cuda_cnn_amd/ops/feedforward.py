@@ -1,0 +1,155 @@
+"""Feed-forward, 8-bit and distillation operators on torch tensors.
+
+Like the rest of ``ops`` they launch on the current stream of the tensors'
+device, allocate their outputs and scratch from torch's caching allocator (so
+they may run on any stream, on any device and inside a captured graph) and
+have no CPU fallback.  They compute no autograd graph: a backward pass is a
+function of its own.
+
+Rows may be strided views (unit stride along the last axis).  The kernels read
+rows in 16-byte pieces: a tensor whose rows are not whole pieces, or not
+aligned to them, is copied into padded rows first (one copy per call).
+"""
+
+from __future__ import annotations
+
+import torch
+
+from .. import _C
+
+_K = _C.kernels
+_GATE = {"none": _K.GATE_NONE, "relu": _K.GATE_RELU, "tanh": _K.GATE_TANH, "silu": _K.GATE_SILU,
+         "gelu": _K.GATE_GELU}
+_ACT = {"none": _K.ACT_NONE, "relu": _K.ACT_RELU, "tanh": _K.ACT_TANH}
+
+
+def _fail(what):
+    raise RuntimeError("mpi_cuda_cnn_amd.ops: " + what)
+
+
+def _matrix(t, name, dtype, shape=None):
+    """Checks that t is a 2-D tensor of dtype (one or a tuple) and, where given, shape."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 2:
+        _fail(f"{name} must be a 2-D tensor")
+    if t.dtype != dtype and not (isinstance(dtype, tuple) and t.dtype in dtype):
+        _fail(f"{name} has dtype {t.dtype}, expected {dtype}")
+    if shape is not None and tuple(t.shape) != shape:
+        _fail(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+
+
+def _vector(t, name, n, dtype=torch.float32):
+    if not isinstance(t, torch.Tensor) or t.dim() != 1 or t.shape[0] != n:
+        _fail(f"{name} must be a vector of {n}")
+    if t.dtype != dtype:
+        _fail(f"{name} has dtype {t.dtype}, expected {dtype}")
+
+
+def _device(first, *more):
+    """The one GPU that all tensors (None: not given) are on."""
+    if not first.is_cuda:
+        _fail("tensors must be on the GPU (no CPU fallback)")
+    dev = first.device
+    for t in more:
+        if t is not None and t.device != dev:
+            _fail(f"tensors on different devices ({dev} and {t.device})")
+    return dev
+
+
+def _pieces(t, n):
+    """(t or a copy, row pitch): rows of whole, aligned 16-byte pieces of n elements, zeros behind the last column."""
+    rows, cols = t.shape
+    if cols % n == 0:
+        ld = t.stride(0) if rows > 1 else cols
+        if t.stride(1) != 1 or ld < cols or ld % n or t.data_ptr() % 16:
+            t = t.clone(memory_format=torch.contiguous_format)
+            ld = cols
+        return t, ld
+    ld = (cols + n - 1) // n * n
+    out = torch.zeros(rows, ld, dtype=t.dtype, device=t.device)
+    out[:, :cols] = t
+    return out, ld
+
+
+def _run(dev, fn, *args):
+    """fn(*args, stream) with dev as the current device (a kernel's launch goes to the current one)."""
+    s = torch.cuda.current_stream(dev).cuda_stream
+    if dev.index == torch.cuda.current_device():
+        fn(*args, s)
+    else:
+        with torch.cuda.device(dev):
+            fn(*args, s)
+
+
+def _gate_kind(act):
+    if act not in _GATE:
+        _fail(f"unknown activation {act!r} (one of {', '.join(_GATE)})")
+    return _GATE[act]
+
+
+def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act: str = "silu", save: bool = False):
+    """h = act(x @ w_gate.T) * (x @ w_up.T): both projections of a gated feed-forward block, the activation and the
+    product in one kernel.
+
+    x [M, D], w_gate, w_up [F, D], bf16; act: none, relu, tanh, silu or gelu (the erf form).  Sums, activation and
+    product are fp32, h [M, F] is rounded once to bf16.  With save=True returns (h, gate, up), the two projections
+    rounded to bf16, which gated_linear_bwd takes."""
+    kind = _gate_kind(act)
+    _matrix(x, "x", torch.bfloat16)
+    M, D = x.shape
+    _matrix(w_gate, "w_gate", torch.bfloat16)
+    F = w_gate.shape[0]
+    _matrix(w_gate, "w_gate", torch.bfloat16, (F, D))
+    _matrix(w_up, "w_up", torch.bfloat16, (F, D))
+    if D == 0 or F == 0:
+        _fail("gated_linear: empty weights")
+    dev = _device(x, w_gate, w_up)
+    h = torch.empty(M, F, dtype=torch.bfloat16, device=dev)
+    gate, up = (torch.empty_like(h), torch.empty_like(h)) if save else (None, None)
+    if M:
+        xa, ldx = _pieces(x, 8)
+        wg, ldw = _pieces(w_gate, 8)
+        wu, ldu = _pieces(w_up, 8)
+        if ldu != ldw:  # both weights are read with one pitch
+            wg, wu, ldw = wg.contiguous(), wu.contiguous(), wg.shape[1]
+        _run(dev, _K.gated_forward, M, D, F, kind, xa.data_ptr(), ldx, wg.data_ptr(), wu.data_ptr(), ldw, h.data_ptr(),
+             gate.data_ptr() if save else 0, up.data_ptr() if save else 0)
+    return (h, gate, up) if save else h
+
+
+def linear_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+              b: torch.Tensor | None = None, act: str = "none", out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """y = act((x @ w.T) * x_scale[:, None] * w_scale + b) on 8-bit integers.
+
+    x [M, K] int8 with a scale per row (token) x_scale [M], w [N, K] int8 with a scale per row (output channel)
+    w_scale [N], b [N] or None, all three fp32; act: none, relu or tanh.  The integer sum is exact in 32 bits
+    (K <= 131071), scaling, bias and activation are fp32, y [M, N] is rounded once to out_dtype (bf16 or fp32)."""
+    if act not in _ACT:
+        _fail(f"unknown activation {act!r} (one of {', '.join(_ACT)})")
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        _fail(f"linear_i8: unsupported out_dtype {out_dtype} (bf16 / fp32)")
+    _matrix(x, "x", torch.int8)
+    M, K = x.shape
+    _matrix(w, "w", torch.int8)
+    N = w.shape[0]
+    _matrix(w, "w", torch.int8, (N, K))
+    if K == 0 or N == 0:
+        _fail("linear_i8: empty weights")
+    if K > _K.LINEAR_I8_MAX_K:
+        _fail(f"linear_i8: K = {K} is over {_K.LINEAR_I8_MAX_K}, the most that 32-bit sums hold exactly")
+    _vector(x_scale, "x_scale", M)
+    _vector(w_scale, "w_scale", N)
+    if b is not None:
+        _vector(b, "b", N)
+    dev = _device(x, x_scale, w, w_scale, b)
+    y = torch.empty(M, N, dtype=out_dtype, device=dev)
+    if M:
+        xa, ldx = _pieces(x, 16)
+        wa, ldw = _pieces(w, 16)
+        sx, sw = x_scale.contiguous(), w_scale.contiguous()
+        bias = b.contiguous() if b is not None else None
+        _run(dev, _K.linear_i8, M, N, K, _ACT[act], xa.data_ptr(), ldx, sx.data_ptr(), wa.data_ptr(), ldw, sw.data_ptr(),
+             bias.data_ptr() if bias is not None else 0, y.data_ptr(), out_dtype == torch.float32)
+    return y
+
+
+__all__ = ["gated_linear", "linear_i8"]
