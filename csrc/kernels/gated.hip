@@ -26,7 +26,7 @@ using tile::Tile;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int A> __device__ __forceinline__ float gate_f(float v) {
-  if constexpr (A == GATE_RELU) return v > 0.f ? v : 0.f * v;  // keeps a NaN
+  if constexpr (A == GATE_RELU) return v < 0.f ? 0.f : v;  // keeps a NaN
   if constexpr (A == GATE_TANH) return tanhf(v);
   if constexpr (A == GATE_SILU) return v / (1.f + __builtin_amdgcn_exp2f(-kLog2e * v));
   if constexpr (A == GATE_GELU) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
@@ -41,22 +41,6 @@ template <class Fn> __host__ __device__ __forceinline__ void with_gate(int act, 
     case GATE_SILU: f(ActK<GATE_SILU>{}); break;
     case GATE_GELU: f(ActK<GATE_GELU>{}); break;
     default: f(ActK<GATE_NONE>{}); break;
-  }
-}
-
-// 16 consecutive outputs of one row from column n on: two stores where the
-// row's pitch keeps 16-byte alignment (`wide`) and all of them exist
-__device__ __forceinline__ void put16(bf16* out, int64_t at, int n, int N, bool wide, const float (&v)[16]) {
-#pragma unroll
-  for (int k = 0; k < 16; k += 8) {
-    if (wide && n + k + 8 <= N) {
-      const bf16x4 a = cvt4(v[k], v[k + 1], v[k + 2], v[k + 3]), b = cvt4(v[k + 4], v[k + 5], v[k + 6], v[k + 7]);
-      store8(out + at + k, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
-    } else {
-#pragma unroll
-      for (int e = k; e < k + 8; ++e)
-        if (n + e < N) out[at + e] = (bf16)v[e];
-    }
   }
 }
 
@@ -83,32 +67,34 @@ __global__ void __launch_bounds__(tile::kThreads, WPE) gated_tile_kernel(GatedPa
   T t;
   t.run(op, lds, f0, m0, 0, (int)((op.kbytes + KS - 1) / KS));
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int r32 = lane & 31, g = lane >> 5, wa = wave >> 1, wb = wave & 1;
-  const int M = p.M, F = p.F;
-  const bool wide = F % 8 == 0;
-  bf16* h = static_cast<bf16*>(p.h);
-  bf16* gate = static_cast<bf16*>(p.gate);
-  bf16* up = static_cast<bf16*>(p.up);
+  const int wave = threadIdx.x >> 6, wa = wave >> 1, wb = wave & 1;
+  const bool wide = p.F % 8 == 0;
+  typedef tile::RowStore<bf16, FA / 2> Rows;
+  const Rows rows{lds + wave * Rows::kBytes};
+  static_assert(4 * Rows::kBytes <= T::kLds, "row buffers fit the images");
+  __syncthreads();  // every wave has read the last image
+  const int f = f0 + T::a_out(wa, 0, 0);
+  float v[16];
 #pragma unroll
-  for (int i = 0; i < FA / 2; ++i) {
-    const int f = f0 + T::a_out(wa, i, g);
+  for (int j = 0; j < FB; ++j) {
+    const int m = m0 + T::b_out(wb, j, 0);
 #pragma unroll
-    for (int j = 0; j < FB; ++j) {
-      const int m = m0 + T::b_out(wb, j, r32);
-      if (m >= M || f >= F) continue;
-      float gv[16], uv[16], hv[16];
+    for (int i = 0; i < FA / 2; ++i) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        gv[e] = t.acc[i][j][e];
-        uv[e] = t.acc[FA / 2 + i][j][e];
-        hv[e] = gate_f<ACT>(gv[e]) * uv[e];
-      }
-      const int64_t at = (int64_t)m * F + f;
-      put16(h, at, f, F, wide, hv);
-      if (gate) {
-        put16(gate, at, f, F, wide, gv);
-        put16(up, at, f, F, wide, uv);
+      for (int e = 0; e < 16; ++e) v[e] = gate_f<ACT>(t.acc[i][j][e]) * t.acc[FA / 2 + i][j][e];
+      rows.put(i, v);
+    }
+    rows.flush(static_cast<bf16*>(p.h), m, f, p.M, p.F, wide);
+    if (p.gate) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int i = 0; i < FA / 2; ++i) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[e] = t.acc[k * (FA / 2) + i][j][e];
+          rows.put(i, v);
+        }
+        rows.flush(static_cast<bf16*>(k ? p.up : p.gate), m, f, p.M, p.F, wide);
       }
     }
   }

@@ -22,30 +22,9 @@ using tile::I8;
 using tile::Operands;
 using tile::Tile;
 
-// 16 consecutive outputs of one row from column n on: 16-byte stores where the
-// row's pitch keeps their alignment (`wide`) and all of them exist
-template <class TO>
-__device__ __forceinline__ void put16(TO* out, int64_t at, int n, int N, bool wide, const float (&v)[16]) {
-#pragma unroll
-  for (int k = 0; k < 16; k += 8) {
-    if (wide && n + k + 8 <= N) {
-      if constexpr (sizeof(TO) == 2) {
-        const bf16x4 a = cvt4(v[k], v[k + 1], v[k + 2], v[k + 3]), b = cvt4(v[k + 4], v[k + 5], v[k + 6], v[k + 7]);
-        store8(out + at + k, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
-      } else {
-        store8(out + at + k, f32x8{v[k], v[k + 1], v[k + 2], v[k + 3], v[k + 4], v[k + 5], v[k + 6], v[k + 7]});
-      }
-    } else {
-#pragma unroll
-      for (int e = k; e < k + 8; ++e)
-        if (n + e < N) out[at + e] = (TO)v[e];
-    }
-  }
-}
-
 // ReLU that keeps a NaN (a row whose scale is NaN stays visible)
 template <int A> __device__ __forceinline__ float act_i8(float v) {
-  if constexpr (A == ACT_RELU) return v > 0.f ? v : 0.f * v;
+  if constexpr (A == ACT_RELU) return v < 0.f ? 0.f : v;
   else return act_c<A>(v);
 }
 
@@ -61,31 +40,44 @@ __global__ void __launch_bounds__(tile::kThreads, WPE) i8_tile_kernel(LinearI8Pa
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r32 = lane & 31, g = lane >> 5, wa = wave >> 1, wb = wave & 1;
-  const int M = p.M, N = p.N;
-  const bool wide = N % 8 == 0;
-  TO* y = static_cast<TO*>(p.y);
-  float sx[FB];
+  const bool wide = p.N % 8 == 0;
+  typedef tile::RowStore<TO, FA> Rows;
+  const Rows rows{lds + wave * Rows::kBytes};
+  // the tile's scales and biases, one of each per thread, dealt out through LDS
+  float* sw = reinterpret_cast<float*>(lds + 4 * Rows::kBytes);
+  float* bias = sw + T::RA;
+  float* sx = bias + T::RA;
+  static_assert(T::RA <= tile::kThreads && T::RB <= tile::kThreads, "one value per thread");
+  static_assert(4 * Rows::kBytes + 4 * (2 * T::RA + T::RB) <= T::kLds, "row buffers and scales fit the images");
+  const int tid = threadIdx.x, n = min(n0 + tid, p.N - 1);
+  const float swv = p.sw[n], bv = p.bias ? p.bias[n] : 0.f, sxv = p.sx[min(m0 + tid, p.M - 1)];
+  __syncthreads();  // every wave has read the last image
+  if (tid < T::RA) {
+    sw[tid] = swv;
+    bias[tid] = bv;
+  }
+  if (tid < T::RB) sx[tid] = sxv;
+  __syncthreads();
+  f32x4 ws[FA][4], wb4[FA][4];
 #pragma unroll
-  for (int j = 0; j < FB; ++j) sx[j] = p.sx[min(m0 + T::b_out(wb, j, r32), M - 1)];
+  for (int i = 0; i < FA; ++i)
 #pragma unroll
-  for (int i = 0; i < FA; ++i) {
-    const int n = n0 + T::a_out(wa, i, g);
-    float sw[16], b[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int c = min(n + e, N - 1);
-      sw[e] = p.sw[c];
-      b[e] = p.bias ? p.bias[c] : 0.f;
+    for (int e = 0; e < 4; ++e) {
+      ws[i][e] = *reinterpret_cast<const f32x4*>(sw + T::a_out(wa, i, g) + 4 * e);
+      wb4[i][e] = *reinterpret_cast<const f32x4*>(bias + T::a_out(wa, i, g) + 4 * e);
     }
 #pragma unroll
-    for (int j = 0; j < FB; ++j) {
-      const int m = m0 + T::b_out(wb, j, r32);
-      if (m >= M || n >= N) continue;
+  for (int j = 0; j < FB; ++j) {
+    const float xs = sx[T::b_out(wb, j, r32)];
+#pragma unroll
+    for (int i = 0; i < FA; ++i) {
       float v[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = act_i8<ACT>((float)t.acc[i][j][e] * (sx[j] * sw[e]) + b[e]);
-      put16(y, (int64_t)m * N + n, n, N, wide, v);
+      for (int e = 0; e < 16; ++e)
+        v[e] = act_i8<ACT>((float)t.acc[i][j][e] * (xs * ws[i][e >> 2][e & 3]) + wb4[i][e >> 2][e & 3]);
+      rows.put(i, v);
     }
+    rows.flush(static_cast<TO*>(p.y), m0 + T::b_out(wb, j, 0), n0 + T::a_out(wa, 0, 0), p.M, p.N, wide);
   }
 }
 
