@@ -37,10 +37,10 @@ ENG_SRC   := $(wildcard csrc/engine/*.cpp)
 ENG_OBJ   := $(patsubst csrc/engine/%.cpp,$(OBJ)/engine/%.o,$(ENG_SRC))
 # headers that only the feed-forward, 8-bit and distillation kernels (and the
 # bindings) read
-FF_HDRS   := csrc/kernels/feedforward.h csrc/kernels/tile_gemm.h csrc/kernels/few_rows.h
+FF_HDRS   := csrc/kernels/feedforward.h csrc/kernels/tile_gemm.h csrc/kernels/few_rows.h csrc/kernels/gate_act.h
 HDRS      := $(filter-out $(FF_HDRS),$(wildcard csrc/include/mcc/*.h csrc/kernels/*.h csrc/apps/*.h)) \
              csrc/core/cpu_kernels.inc
-FF_OBJ    := $(patsubst %,$(OBJ)/kernels/%.o,gated linear_i8) $(OBJ)/bindings/module.o
+FF_OBJ    := $(patsubst %,$(OBJ)/kernels/%.o,gated gated_bwd linear_i8 rmsnorm_i8 distill) $(OBJ)/bindings/module.o
 
 MODULE    := mpi_cuda_cnn_amd/_C$(EXT)
 BINS      := build/bin/cnn build/bin/cnn_hip build/bin/cnn_dist build/bin/test_watchdog build/bin/test_comm
@@ -70,10 +70,10 @@ $(OBJ)/kernels/%.o: csrc/kernels/%.hip $(HDRS)
 	$(HIPCC) $(HIPFLAGS) -c $< -o $@
 
 $(FF_OBJ): $(FF_HDRS)
-# gated, linear_i8: the source order of their tile loop is the schedule; the
+# gated, gated_bwd, linear_i8: the source order of their tile loop is the schedule; the
 # scheduler before register allocation would move the MFMAs and, with all 256
 # accumulation registers in use, pay in ~270 register moves a step
-$(OBJ)/kernels/gated.o $(OBJ)/kernels/linear_i8.o: HIPFLAGS += -mllvm -enable-misched=0
+$(OBJ)/kernels/gated.o $(OBJ)/kernels/gated_bwd.o $(OBJ)/kernels/linear_i8.o: HIPFLAGS += -mllvm -enable-misched=0
 
 # lenet.hip: MFMA results in VGPRs (no v_accvgpr_read per accumulator in the
 # VALU-bound epilogues; the register file is unified on gfx950)

@@ -680,6 +680,49 @@ PYBIND11_MODULE(_C, m) {
         py::arg("M"), py::arg("N"), py::arg("K"), py::arg("act"), py::arg("x"), py::arg("ldx"), py::arg("sx"),
         py::arg("w"), py::arg("ldw"), py::arg("sw"), py::arg("bias"), py::arg("y"), py::arg("f32"),
         py::arg("stream") = 0);
+  k.def("gated_backward_bytes", &gpu::gated_backward_bytes, py::arg("M"), py::arg("D"), py::arg("F"));
+  k.def("gated_backward",
+        [](int M, int D, int F, int act, uintptr_t dh, uintptr_t gate, uintptr_t up, uintptr_t x, int64_t ldx, uintptr_t wg,
+           uintptr_t wu, int64_t ldw, uintptr_t dx, uintptr_t dw, uintptr_t work, uintptr_t s) {
+          gpu::GatedBwdParams p;
+          p.M = M; p.D = D; p.F = F; p.act = act;
+          p.dh = ptr<void>(dh); p.gate = ptr<void>(gate); p.up = ptr<void>(up);
+          p.x = ptr<void>(x); p.ldx = ldx;
+          p.wg = ptr<void>(wg); p.wu = ptr<void>(wu); p.ldw = ldw;
+          p.dx = ptr<void>(dx); p.dw = ptr<void>(dw); p.work = ptr<void>(work);
+          gpu::gated_backward(p, stream_of(s));
+        },
+        py::arg("M"), py::arg("D"), py::arg("F"), py::arg("act"), py::arg("dh"), py::arg("gate"), py::arg("up"),
+        py::arg("x"), py::arg("ldx"), py::arg("wg"), py::arg("wu"), py::arg("ldw"), py::arg("dx"), py::arg("dw"),
+        py::arg("work"), py::arg("stream") = 0);
+  k.def("rmsnorm_i8",
+        [](int M, int D, bool f32, uintptr_t x, int64_t ldx, uintptr_t r, int64_t ldr, uintptr_t w, float eps,
+           uintptr_t sum, uintptr_t q, uintptr_t scale, uintptr_t s) {
+          gpu::RmsnormI8Params p;
+          p.M = M; p.D = D; p.f32 = f32; p.eps = eps;
+          p.x = ptr<void>(x); p.ldx = ldx; p.r = ptr<void>(r); p.ldr = ldr; p.w = ptr<void>(w);
+          p.sum = ptr<void>(sum); p.q = ptr<int8_t>(q); p.scale = ptr<float>(scale);
+          gpu::rmsnorm_i8(p, stream_of(s));
+        },
+        py::arg("M"), py::arg("D"), py::arg("f32"), py::arg("x"), py::arg("ldx"), py::arg("r"), py::arg("ldr"),
+        py::arg("w"), py::arg("eps"), py::arg("sum"), py::arg("q"), py::arg("scale"), py::arg("stream") = 0);
+  k.def("distill_bytes", &gpu::distill_bytes, py::arg("M"), py::arg("N"), py::arg("z_f32"));
+  k.def("distill_kl",
+        [](int M, int N, int K, uintptr_t z, int64_t ldz, bool z_f32, uintptr_t t, bool t_f32, uintptr_t idx, bool idx64,
+           float temperature, float scale, uintptr_t dz, bool dz_f32, uintptr_t loss, uintptr_t work, uintptr_t s) {
+          gpu::DistillParams p;
+          p.M = M; p.N = N; p.K = K;
+          p.z = ptr<void>(z); p.ldz = ldz; p.z_f32 = z_f32;
+          p.t = ptr<void>(t); p.t_f32 = t_f32; p.idx = ptr<void>(idx); p.idx64 = idx64;
+          p.temperature = temperature; p.scale = scale;
+          p.dz = ptr<void>(dz); p.dz_f32 = dz_f32; p.loss = ptr<float>(loss); p.work = ptr<void>(work);
+          gpu::distill_kl(p, stream_of(s));
+        },
+        py::arg("M"), py::arg("N"), py::arg("K"), py::arg("z"), py::arg("ldz"), py::arg("z_f32"), py::arg("t"),
+        py::arg("t_f32"), py::arg("idx"), py::arg("idx64"), py::arg("temperature"), py::arg("scale"), py::arg("dz"),
+        py::arg("dz_f32"), py::arg("loss"), py::arg("work"), py::arg("stream") = 0);
+  k.attr("RMSNORM_I8_MAX_D") = gpu::kRmsnormI8MaxD;
+  k.attr("DISTILL_MAX_K") = gpu::kDistillMaxK;
   k.attr("GATE_NONE") = (int)gpu::GATE_NONE;
   k.attr("GATE_RELU") = (int)gpu::GATE_RELU;
   k.attr("GATE_TANH") = (int)gpu::GATE_TANH;

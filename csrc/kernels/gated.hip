@@ -9,6 +9,7 @@
 // training step keeps.
 #include "feedforward.h"
 #include "few_rows.h"
+#include "gate_act.h"
 #include "kernels.h"
 #include "mcc/common.h"
 #include "tile_gemm.h"
@@ -22,27 +23,6 @@ using tile::Bf16;
 using tile::FewRows;
 using tile::Operands;
 using tile::Tile;
-
-constexpr float kLog2e = 1.4426950408889634f;
-
-template <int A> __device__ __forceinline__ float gate_f(float v) {
-  if constexpr (A == GATE_RELU) return v < 0.f ? 0.f : v;  // keeps a NaN
-  if constexpr (A == GATE_TANH) return tanhf(v);
-  if constexpr (A == GATE_SILU) return v / (1.f + __builtin_amdgcn_exp2f(-kLog2e * v));
-  if constexpr (A == GATE_GELU) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
-  return v;
-}
-
-// calls f with the activation as a compile-time constant
-template <class Fn> __host__ __device__ __forceinline__ void with_gate(int act, Fn&& f) {
-  switch (act) {
-    case GATE_RELU: f(ActK<GATE_RELU>{}); break;
-    case GATE_TANH: f(ActK<GATE_TANH>{}); break;
-    case GATE_SILU: f(ActK<GATE_SILU>{}); break;
-    case GATE_GELU: f(ActK<GATE_GELU>{}); break;
-    default: f(ActK<GATE_NONE>{}); break;
-  }
-}
 
 Operands operands(const GatedParams& p) {
   Operands o;

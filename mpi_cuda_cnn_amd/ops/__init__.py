@@ -15,7 +15,10 @@ fail loudly on CPU tensors: there is no eager fallback.
     conv2d_dgrad_nhwc(dy, w, ...)   dx of a stride-1 conv (the same kernel on flipped weights)
     conv2d_wgrad_nhwc(dy, x, ...)   (dW OIHW fp32, db fp32) split-K implicit GEMM
     gated_linear(x, wg, wu, act)    act(x @ wg.T) * (x @ wu.T)       (one kernel; feedforward.py)
+    gated_linear_bwd(dh, x, wg, wu, gate, up, act) its dx, dwg, dwu
     linear_i8(xq, sx, wq, sw, b, act) act((xq @ wq.T) * sx * sw + b) (int8 MFMA, exact 32-bit sums)
+    rmsnorm_i8(x, w, residual)      int8 rows and scales of RMS norm(x + residual), and the sum
+    distill_kl(z, t, idx, T)        dlogits, loss from a teacher's top logits
 
 Reference counterparts: Layer_feedForw_full / Layer_feedBack_full
 (cnn.c:113-173), Layer_feedForw_conv / Layer_feedBack_conv (cnn.c:175-247) and
@@ -28,7 +31,7 @@ from __future__ import annotations
 import torch
 
 from .. import _C
-from .feedforward import gated_linear, linear_i8  # noqa: F401
+from .feedforward import distill_kl, gated_linear, gated_linear_bwd, linear_i8, rmsnorm_i8
 
 _K = _C.kernels
 _ACT = {"none": _K.ACT_NONE, "relu": _K.ACT_RELU, "tanh": _K.ACT_TANH}
@@ -235,4 +238,5 @@ def conv2d_wgrad_nhwc(dy: torch.Tensor, x: torch.Tensor, KS: int, stride: int = 
 
 
 __all__ = ["linear", "linear_dgrad", "linear_wgrad", "softmax_xent", "sgd_", "conv2d_nhwc", "conv2d_dgrad_nhwc",
-           "conv2d_wgrad_nhwc", "pack_conv_weight", "gated_linear", "linear_i8"]
+           "conv2d_wgrad_nhwc", "pack_conv_weight", "gated_linear", "gated_linear_bwd", "linear_i8",
+           "rmsnorm_i8", "distill_kl"]

@@ -152,4 +152,125 @@ def linear_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     return y
 
 
-__all__ = ["gated_linear", "linear_i8"]
+def _strided(t):
+    """(t or a copy, row pitch): unit stride along the columns."""
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < cols:
+        t = t.contiguous()
+    return t, t.stride(0) if rows > 1 else cols
+
+
+def gated_linear_bwd(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, gate: torch.Tensor,
+                     up: torch.Tensor, act: str = "silu"):
+    """(dx [M, D], dw_gate [F, D], dw_up [F, D]), bf16, of gated_linear from dh [M, F] and the (gate, up) that it saved.
+
+    The gradients of the two projections are rounded to bf16, the matrix unit's operand type; sums are fp32 in a fixed
+    order (the same call gives the same bits)."""
+    kind = _gate_kind(act)
+    _matrix(x, "x", torch.bfloat16)
+    M, D = x.shape
+    _matrix(w_gate, "w_gate", torch.bfloat16)
+    F = w_gate.shape[0]
+    _matrix(w_gate, "w_gate", torch.bfloat16, (F, D))
+    _matrix(w_up, "w_up", torch.bfloat16, (F, D))
+    for t, name in ((dh, "dh"), (gate, "gate"), (up, "up")):
+        _matrix(t, name, torch.bfloat16, (M, F))
+    if D == 0 or F == 0:
+        _fail("gated_linear_bwd: empty weights")
+    dev = _device(x, w_gate, w_up, dh, gate, up)
+    dx = torch.empty(M, D, dtype=torch.bfloat16, device=dev)
+    if M == 0:
+        return dx, torch.zeros_like(w_gate, memory_format=torch.contiguous_format), torch.zeros_like(
+            w_up, memory_format=torch.contiguous_format)
+    dw = torch.empty(2, F, D, dtype=torch.bfloat16, device=dev)
+    work = torch.empty(_K.gated_backward_bytes(M, D, F), dtype=torch.uint8, device=dev)
+    dh, gate, up = dh.contiguous(), gate.contiguous(), up.contiguous()
+    xa, ldx = _strided(x)
+    wg, ldw = _strided(w_gate)
+    wu, ldu = _strided(w_up)
+    if ldu != ldw:
+        wg, wu, ldw = wg.contiguous(), wu.contiguous(), D
+    _run(dev, _K.gated_backward, M, D, F, kind, dh.data_ptr(), gate.data_ptr(), up.data_ptr(), xa.data_ptr(), ldx,
+         wg.data_ptr(), wu.data_ptr(), ldw, dx.data_ptr(), dw.data_ptr(), work.data_ptr())
+    return dx, dw[0], dw[1]
+
+
+def rmsnorm_i8(x: torch.Tensor, w: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6):
+    """(q, scale, s): s = x + residual, y = s * w / sqrt(mean(s**2) + eps) quantised per row to 8 bits.
+
+    x, residual [M, D], w [D], all bf16 or all fp32, D <= 32768.  scale [M] fp32 = max|y| / 127 and q [M, D] int8 =
+    y / scale rounded to nearest even: linear_i8's x and x_scale.  s [M, D] in x's type, from which the norm is NOT
+    taken again (it is of the unrounded sum); without a residual s is x.  A row of zeros has scale 0; a row that holds
+    a value that is not finite, or overflows the fp32 sum of squares, has scale NaN and q = 0, so what is computed
+    from it is NaN.  Inference only: an 8-bit output has no gradient."""
+    if not isinstance(x, torch.Tensor) or x.dtype not in (torch.bfloat16, torch.float32):
+        _fail("x must be a bf16 or fp32 tensor")
+    _matrix(x, "x", x.dtype)
+    M, D = x.shape
+    if D == 0 or D > _K.RMSNORM_I8_MAX_D:
+        _fail(f"rmsnorm_i8: rows of 1 to {_K.RMSNORM_I8_MAX_D} values, got {D}")
+    _vector(w, "w", D, x.dtype)
+    if residual is not None:
+        _matrix(residual, "residual", x.dtype, (M, D))
+    if not eps >= 0:
+        _fail(f"rmsnorm_i8: eps = {eps} must not be negative")
+    dev = _device(x, w, residual)
+    q = torch.empty(M, D, dtype=torch.int8, device=dev)
+    scale = torch.empty(M, dtype=torch.float32, device=dev)
+    s = x if residual is None else torch.empty(M, D, dtype=x.dtype, device=dev)
+    if M:
+        xa, ldx = _strided(x)
+        ra, ldr = _strided(residual) if residual is not None else (None, 0)
+        wa = w.contiguous()
+        _run(dev, _K.rmsnorm_i8, M, D, x.dtype == torch.float32, xa.data_ptr(), ldx, ra.data_ptr() if ra is not None else 0,
+             ldr, wa.data_ptr(), eps, s.data_ptr() if ra is not None else 0, q.data_ptr(), scale.data_ptr())
+    return q, scale, s
+
+
+def distill_kl(logits: torch.Tensor, t_logits: torch.Tensor, t_index: torch.Tensor, temperature: float = 1.0,
+               scale: float = 1.0, grad: bool = True, grad_dtype: torch.dtype | None = None):
+    """(dlogits, loss): distillation from a teacher's top logits, forward and backward in one call.
+
+    logits [M, N] (the student's, bf16 or fp32); row m of t_logits [M, K] (bf16 or fp32) holds the teacher's logits of
+    the classes t_index [M, K] (int32 or int64), K <= 1024, in any order.  An entry whose class is not in [0, N) (say
+    -1) or whose logit is -inf is not there; classes that occur twice add up.  With T = temperature,
+    q = softmax(t_logits[m] / T) over the entries that are there and p = softmax(logits[m] / T):
+
+        loss[m]    = T**2 * sum_k q_k (log q_k - log p[t_index[m, k]])            fp32 [M]
+        dlogits[m] = scale * T * (p - q scattered to its classes)                 [M, N]
+
+    A row without entries has loss 0 and gradient 0.  dlogits is the gradient of scale * loss.sum(), in grad_dtype
+    (default: the logits' type; fp32 logits have fp32 gradients); None with grad=False."""
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in (torch.bfloat16, torch.float32):
+        _fail("logits must be a bf16 or fp32 tensor")
+    _matrix(logits, "logits", logits.dtype)
+    M, N = logits.shape
+    if N == 0:
+        _fail("distill_kl: no classes")
+    _matrix(t_logits, "t_logits", (torch.bfloat16, torch.float32))
+    K = t_logits.shape[1]
+    _matrix(t_logits, "t_logits", (torch.bfloat16, torch.float32), (M, K))
+    _matrix(t_index, "t_index", (torch.int32, torch.int64), (M, K))
+    if K > _K.DISTILL_MAX_K:
+        _fail(f"distill_kl: at most {_K.DISTILL_MAX_K} entries per row, got {K}")
+    if not (0.0 < temperature < float("inf")):
+        _fail(f"distill_kl: temperature = {temperature} must be positive and finite")
+    out = logits.dtype if grad_dtype is None else grad_dtype
+    if out not in (torch.float32, logits.dtype):
+        _fail(f"distill_kl: unsupported grad_dtype {out} (fp32 or the logits' type)")
+    dev = _device(logits, t_logits, t_index)
+    dz = torch.empty(M, N, dtype=out, device=dev) if grad else None
+    loss = torch.empty(M, dtype=torch.float32, device=dev)
+    if M:
+        f32 = logits.dtype == torch.float32
+        za, ldz = _strided(logits)
+        tl, ti = t_logits.contiguous(), t_index.contiguous()
+        nbytes = _K.distill_bytes(M, N, f32)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        _run(dev, _K.distill_kl, M, N, K, za.data_ptr(), ldz, f32, tl.data_ptr(), tl.dtype == torch.float32, ti.data_ptr(),
+             ti.dtype == torch.int64, temperature, scale, dz.data_ptr() if grad else 0, out == torch.float32,
+             loss.data_ptr(), work.data_ptr() if nbytes else 0)
+    return dz, loss
+
+
+__all__ = ["gated_linear", "gated_linear_bwd", "linear_i8", "rmsnorm_i8", "distill_kl"]

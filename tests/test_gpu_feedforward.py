@@ -164,3 +164,299 @@ def test_linear_i8_longest_sum_is_exact(cuda, M, N, K):
 def test_linear_i8_epilogues(cuda, M, N, K, out, act):
     x, sx, w, sw, b = i8_case(gen(5, cuda), M, N, K)
     i8_check(x, sx, w, sw, b, act, ops.linear_i8(x, sx, w, sw, b, act, out_dtype=out))
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# gated_linear_bwd
+# ---------------------------------------------------------------------------------------------------------------
+def gated_bwd_check(dh, x, wg, wu, gate, up, act, out):
+    DH, X, Wg, Wu, G, U = (t.to(D64) for t in (dh, x, wg, wu, gate, up))
+    f, df = act64(G, act)
+    # f and f' carry a few units in the last place of terms of size |f| + 1.13 and |G f''| <= 1
+    dg, eg = DH * U * df, EPS_ACT * (DH * U).abs() * (1.13 + G.abs() * 2.0**-3)
+    du, eu = DH * f, EPS_ACT * DH.abs() * (f.abs() + G.abs() * 2.0**-3)
+    # the projections' gradients are rounded to bf16
+    eg = eg + EPS_BF16 * (dg.abs() + eg) + 1e-38
+    eu = eu + EPS_BF16 * (du.abs() + eu) + 1e-38
+    M, F = dh.shape
+
+    def one(got, ref, err, what):
+        within(got, ref, err + EPS_BF16 * (ref.abs() + err) + 1e-38, what)
+
+    mag = dg.abs() @ Wg.abs() + du.abs() @ Wu.abs()
+    one(out[0], dg @ Wg + du @ Wu, eg @ Wg.abs() + eu @ Wu.abs() + 1.01 * (2 * F + 64) * EPS_SUM * mag, "dx")
+    one(out[1], dg.t() @ X, eg.t() @ X.abs() + 1.01 * (M + 64) * EPS_SUM * (dg.abs().t() @ X.abs()), "dw_gate")
+    one(out[2], du.t() @ X, eu.t() @ X.abs() + 1.01 * (M + 64) * EPS_SUM * (du.abs().t() @ X.abs()), "dw_up")
+
+
+def gated_bwd_case(g, M, D, F, std=1.0):
+    x, wg, wu = randn(g, M, D, std=std), randn(g, F, D, std=D**-0.5), randn(g, F, D, std=D**-0.5)
+    gate, up = (x.float() @ wg.float().t()).bfloat16(), (x.float() @ wu.float().t()).bfloat16()
+    return randn(g, M, F, std=0.1), x, wg, wu, gate, up
+
+
+GATED_BWD = [(1, 64, 16), (1, 1, 1), (2, 136, 70), (3, 9, 1), (16, 512, 100), (17, 264, 33), (33, 72, 257), (64, 4104, 48),
+             (64, 128, 3000), (65, 64, 64), (66, 1, 5), (100, 333, 129), (128, 128, 64), (129, 192, 65), (300, 200, 515),
+             (1000, 520, 130), (4100, 64, 1030), (700, 4360, 4200)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,D,F", GATED_BWD)
+def test_gated_linear_bwd(cuda, M, D, F):
+    case = gated_bwd_case(gen(M * 7 + D + F, cuda), M, D, F)
+    gated_bwd_check(*case, "silu", ops.gated_linear_bwd(*case, "silu"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["none", "relu", "tanh", "silu", "gelu"])
+@pytest.mark.parametrize("M,D,F", [(5, 96, 40), (200, 96, 72)])
+def test_gated_linear_bwd_activations(cuda, M, D, F, act):
+    case = gated_bwd_case(gen(9, cuda), M, D, F, std=3.0)
+    gated_bwd_check(*case, act, ops.gated_linear_bwd(*case, act))
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "tanh", "silu", "gelu"])
+def test_slopes_are_those_of_the_activations(act):
+    """act64's slope, which the backward tests use, against differences in 64 bits."""
+    v = torch.linspace(-9, 9, 2001, dtype=D64) + 1e-3
+    h = 1e-5
+    num = (act64(v + h, act)[0] - act64(v - h, act)[0]) / (2 * h)
+    # third derivatives of all of them are below 4: h^2 / 6 * 4, and 2 roundings of values up to 9 over 2 h
+    assert (num - act64(v, act)[1]).abs().max().item() < h * h + 9 * 2.0**-52 / h
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["silu", "gelu", "tanh"])
+def test_gated_gradient_against_differences(cuda, act):
+    """The whole backward pass against differences of the forward definition in 64 bits."""
+    g = gen(11, cuda)
+    M, D, F = 6, 24, 40
+    x, wg, wu = randn(g, M, D), randn(g, F, D, std=0.3), randn(g, F, D, std=0.3)
+    _, gate, up = ops.gated_linear(x, wg, wu, act, save=True)
+    dh = randn(g, M, F)
+    got = ops.gated_linear_bwd(dh, x, wg, wu, gate, up, act)
+    leaves = [t.to(D64) for t in (x, wg, wu)]
+
+    def value(x, wg, wu):
+        return (dh.to(D64) * act64(x @ wg.t(), act)[0] * (x @ wu.t())).sum().item()
+
+    h = 1e-6
+    for i, leaf in enumerate(leaves):
+        for _ in range(12):
+            at = tuple(int(torch.randint(n, (1,), device=cuda, generator=g)) for n in leaf.shape)
+            side = []
+            for sign in (1, -1):
+                moved = [t.clone() for t in leaves]
+                moved[i][at] += sign * h
+                side.append(value(*moved))
+            num = (side[0] - side[1]) / (2 * h)
+            # saved projections, dG / dU and the gradient itself are rounded to bf16: each term of the sums is off by
+            # at most 2^-8 for dG / dU, and by 2^-8 of its projections' size (|f''| <= 1.6) for the saved ones
+            dxs, a, b = dh.to(D64), leaves[0] @ leaves[1].t(), leaves[0] @ leaves[2].t()
+            f, df = act64(a, act)
+            tg = EPS_BF16 * dxs.abs() * ((b * df).abs() * 2 + b.abs() * 1.6 * a.abs())
+            tu = EPS_BF16 * dxs.abs() * (f.abs() + 1.13 * a.abs())
+            bound = {0: tg @ leaves[1].abs() + tu @ leaves[2].abs(), 1: tg.t() @ leaves[0].abs(),
+                     2: tu.t() @ leaves[0].abs()}[i][at].item()
+            assert abs(got[i][at].item() - num) <= 1.05 * bound + EPS_BF16 * abs(num) + 1e-6, (i, at)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# rmsnorm_i8
+# ---------------------------------------------------------------------------------------------------------------
+def norm_check(x, w, r, eps, out):
+    q, scale, s = out
+    v = x.to(D64) + (r.to(D64) if r is not None else 0.0)
+    D = x.shape[1]
+    y = v / torch.sqrt((v * v).mean(1, keepdim=True) + eps) * w.to(D64)
+    # the fp32 sum v has one rounding; the mean's D additions weigh half in the root
+    rel = EPS_F32 * 8 + D * EPS_F32 * 0.5
+    top = y.abs().amax(1)
+    within(scale, top / 127, rel * top / 127 + 1e-45, "scale")
+    if r is not None:
+        eps_s = EPS_BF16 if s.dtype == torch.bfloat16 else EPS_F32
+        within(s, v, 1.01 * eps_s * v.abs() + EPS_F32 * v.abs() + 1e-38, "s")
+    else:
+        assert s is x
+    # q: the nearest integer of y / scale, whose own error is a few 2^-24 of at most 127
+    z = y / (top / 127).clamp(min=1e-300)[:, None]
+    assert (q.to(D64) - z).abs().max().item() <= 0.5 + 127 * 8 * EPS_F32
+    # (the factor 1 / rms cancels in q: no error of the mean in it)
+    assert q.to(torch.int32).abs().max().item() <= 127
+
+
+NORM = [(1, 1), (1, 8), (3, 7), (5, 64), (4, 512), (9, 513), (2, 1000), (7, 1024), (3, 1025), (2, 2048), (3, 2056), (1, 4096),
+        (33, 4100), (3, 8192), (2, 8193), (2, 16384), (3, 20001), (2, 32768), (1000, 96), (20000, 17)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,D", NORM)
+def test_rmsnorm_i8(cuda, M, D, dtype):
+    g = gen(M + D, cuda)
+    x, r = randn(g, M, D, dtype=dtype), randn(g, M, D, std=5.0, dtype=dtype)
+    w = (1 + 0.2 * torch.randn(D, device=cuda, generator=g)).to(dtype)
+    norm_check(x, w, r, 1e-6, ops.rmsnorm_i8(x, w, r))
+    norm_check(x, w, None, 1e-5, ops.rmsnorm_i8(x, w, eps=1e-5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [100, 3000, 16000])
+def test_rmsnorm_i8_special_rows(cuda, D):
+    """Rows of zeros, of values that are not finite, of tiny and of huge ones; no row touches another."""
+    g = gen(2, cuda)
+    x = randn(g, 9, D, dtype=torch.float32)
+    x[0] = 0
+    x[2, D // 2] = float("nan")
+    x[3, 1] = float("inf")
+    x[4, D - 1] = -float("inf")
+    x[5] *= 1e-30
+    x[6] *= 1e18 / D**0.5
+    x[7] *= 1e30  # the squares overflow
+    w = torch.ones(D, device=cuda)
+    q, scale, s = ops.rmsnorm_i8(x, w, torch.zeros_like(x))
+    assert torch.equal(s.isnan(), x.isnan()) and torch.equal(s.nan_to_num(), x.nan_to_num())
+    assert scale[0].item() == 0 and not q[0].any()
+    for row in (2, 3, 4, 7):
+        assert math.isnan(scale[row].item()) and not q[row].any(), row
+    for row in (1, 5, 6, 8):
+        one = ops.rmsnorm_i8(x[row : row + 1], w)
+        v = x[row : row + 1]
+        norm_check(v, w, None, 1e-6, ops.rmsnorm_i8(v, w))
+        assert torch.equal(one[0][0], q[row]) and torch.equal(one[1][0], scale[row]), row
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# distill_kl
+# ---------------------------------------------------------------------------------------------------------------
+def distill64(z, tv, ti, T, scale):
+    """(dz, loss, p, log terms' size) in 64 bits."""
+    M, N = z.shape
+    logp = torch.log_softmax(z.to(D64) / T, 1)
+    there = (ti >= 0) & (ti < N) & (tv != -math.inf)
+    some = there.any(1, keepdim=True)
+    t = torch.where(there, tv.to(D64) / T, torch.full_like(tv, -math.inf, dtype=D64))
+    t = torch.where(some, t, torch.zeros_like(t))
+    logq = torch.log_softmax(t, 1)
+    q = torch.where(there, torch.exp(logq), torch.zeros_like(logq))
+    at = torch.where(there, ti.long(), torch.zeros_like(ti.long()))
+    lp = logp.gather(1, at)
+    terms = torch.where(q > 0, q * (torch.where(q > 0, logq, torch.zeros_like(logq)) - lp), torch.zeros_like(q))
+    p = torch.exp(logp)
+    sq = torch.zeros_like(p).scatter_add_(1, at, q)
+    dz = torch.where(some, scale * T * (p - sq), torch.zeros_like(p))
+    size = torch.where(q > 0, q * (logq.abs() + lp.abs()), torch.zeros_like(q)).sum(1)
+    return dz, T * T * terms.sum(1), p, sq, T * T * size
+
+
+def distill_check(z, tv, ti, T, scale, dz, loss):
+    ref, rl, p, sq, size = distill64(z, tv, ti, T, scale)
+    zf = z.to(D64)
+    N = z.shape[1]
+    zmax = zf.amax(1, keepdim=True)
+    # exponent (z - max) log2(e) / T: three roundings of its size; the sum of N terms in at most N / 64 + 64 steps
+    # that do not cancel; exp2, the division and the products a few units
+    arg = torch.where(torch.isfinite(zf), (zmax - zf) / T, torch.zeros_like(zf))
+    rel_e = EPS_F32 * (4 * arg + 8)
+    rel_s = (p * rel_e).sum(1, keepdim=True) + EPS_F32 * (N / 64 + 64)
+    if dz is not None:
+        err = scale * T * (p * (rel_e + rel_s) + sq * 64 * EPS_F32)
+        eps = EPS_BF16 if dz.dtype == torch.bfloat16 else EPS_F32
+        within(dz, ref, err + 1.01 * eps * (ref.abs() + err) + 1e-38, "dz")
+    K = tv.shape[1]
+    lerr = (64 + K) * EPS_F32 * size + T * T * (rel_s[:, 0] + EPS_F32 * 8 * (zmax.abs()[:, 0] / T + 1))
+    within(loss, rl, lerr + 1e-38, "loss")
+
+
+def distill_case(g, M, N, K, dtype=torch.float32, index=torch.int64, std=2.0):
+    dev = g.device
+    z = randn(g, M, N, std=std, dtype=dtype)
+    tv = randn(g, M, K, std=3.0, dtype=dtype)
+    ti = torch.randint(0, N, (M, K), device=dev, generator=g).to(index)
+    drop = torch.rand(M, K, device=dev, generator=g) < 0.2
+    ti[drop] = -1
+    return z, tv, ti
+
+
+DISTILL = [(1, 1, 1), (1, 10, 3), (3, 2, 2), (5, 100, 10), (640, 1000, 10), (9, 1017, 64), (4, 1018, 5), (3, 4089, 33),
+           (2, 4090, 7), (3, 8185, 16), (2, 8186, 1), (130, 16377, 12), (129, 16378, 12), (130, 32770, 20), (3, 50001, 64),
+           (131, 65001, 9), (130, 65529, 9), (129, 65530, 9), (1, 131072, 40), (140, 131065, 5), (2, 250001, 64)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,N,K", DISTILL)
+def test_distill_kl(cuda, M, N, K, dtype):
+    z, tv, ti = distill_case(gen(M + N + K, cuda), M, N, K, dtype)
+    dz, loss = ops.distill_kl(z, tv, ti, temperature=2.0, scale=0.5)
+    assert dz.dtype == dtype
+    distill_check(z, tv, ti, 2.0, 0.5, dz, loss)
+    none, alone = ops.distill_kl(z, tv, ti, temperature=2.0, grad=False)
+    assert none is None and torch.equal(alone, loss)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(70, 37, 1024), (3, 5000, 1024), (2, 70000, 700)])
+def test_distill_kl_many_entries_and_types(cuda, M, N, K):
+    """Classes that occur many times add up; int32 classes, other types of teacher and gradient."""
+    z, tv, ti = distill_case(gen(1, cuda), M, N, K, torch.bfloat16, torch.int32)
+    dz, loss = ops.distill_kl(z, tv.float(), ti, grad_dtype=torch.float32)
+    assert dz.dtype == torch.float32
+    # a sum of up to K shares of one class
+    ref, rl, p, sq, size = distill64(z, tv.float(), ti, 1.0, 1.0)
+    assert (dz.to(D64) - ref).abs().max().item() < (K + 200) * EPS_F32
+    distill_check(z, tv.float(), ti, 1.0, 1.0, None, loss)
+    again = ops.distill_kl(z, tv.float(), ti, grad_dtype=torch.float32)
+    assert torch.equal(dz, again[0]) and torch.equal(loss, again[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [50, 3000, 20000, 40000, 140000])
+def test_distill_kl_masks(cuda, N):
+    """Rows without entries, entries out of range or of -inf, masked classes, the type's lowest value."""
+    low = torch.finfo(torch.float32).min
+    z, tv, ti = distill_case(gen(4, cuda), 9, N, 6)
+    ti = torch.where(ti < 0, ti + 1, ti)  # all there
+    ti[0] = -1
+    ti[1] = torch.tensor([N, -7, 2**40, -(2**40), N + 1, -1], device=cuda)
+    tv[2] = -math.inf
+    tv[3, :5] = -math.inf
+    tv[4, ::2] = low
+    tv[5] = low
+    z[6, : N // 2] = -math.inf
+    ti[6] = N - 1 - torch.arange(6, device=cuda)
+    z[7, : N // 2] = low
+    ti[7] = N - 1 - torch.arange(6, device=cuda)
+    tv[8, 3] = float("nan")
+    ti[8, 3] = -1  # a NaN that is not there
+    dz, loss = ops.distill_kl(z, tv, ti, temperature=1.5)
+    for row in (0, 1, 2):
+        assert loss[row].item() == 0 and not dz[row].any(), row
+    tv[8, 3] = 0.0
+    distill_check(z[3:], tv[3:], ti[3:], 1.5, 1.0, dz[3:], loss[3:])
+
+
+@pytest.mark.gpu
+def test_distill_kl_no_entries_at_all(cuda):
+    z = randn(gen(1, cuda), 4, 100)
+    dz, loss = ops.distill_kl(z, torch.empty(4, 0, device=cuda), torch.empty(4, 0, dtype=torch.int64, device=cuda))
+    assert not dz.any() and not loss.any()
+
+
+@pytest.mark.gpu
+def test_distill_gradient_against_differences(cuda):
+    g = gen(6, cuda)
+    z, tv, ti = distill_case(g, 3, 40, 8)
+    T = 2.0
+    dz, _ = ops.distill_kl(z, tv, ti, temperature=T, scale=0.25)
+    h = 1e-5
+    for _ in range(30):
+        at = (int(torch.randint(3, (1,), device=cuda, generator=g)), int(torch.randint(40, (1,), device=cuda, generator=g)))
+        side = []
+        for sign in (1, -1):
+            m = z.to(D64)
+            m[at] += sign * h
+            side.append(0.25 * distill64(m, tv, ti, T, 1.0)[1].sum().item())
+        num = (side[0] - side[1]) / (2 * h)
+        # h^2 / 6 of a third derivative below 1, the differences' rounding, and fp32 in the kernel
+        assert abs(dz[at].item() - num) < h * h + 1e-15 / h * 100 + 1e-6
