@@ -16,13 +16,9 @@
 //
 // Workgroup: 4 waves in 2 x 2, wave tile (32 FA) x (32 FB), workgroup tile
 // (64 FA) x (64 FB).  Operands go HBM -> LDS by global_load_lds (16 bytes a
-// lane) into NST images of KS bytes of K; the fragments of one depth are read
-// while those of the depth before are multiplied, and the last depth of a step
-//
-//   waits for this wave's reads of image kt and its loads of step kt+1,
-//   passes the step's one barrier (now every wave has read image kt),
-//   loads step kt+NST into the place of image kt,
-//   reads depth 0 of step kt+1 and multiplies.
+// lane) into NST images of KS bytes of K, image kt + NST into the place of image
+// kt; how reads, loads and waits are dealt out among a step's MFMAs stands at
+// `step` below.
 //
 // At 4 x 4 fragments a wave multiplies 2048 cycles per 128 bytes of K while the
 // four waves read 128 KiB of LDS (1024 cycles at 128 B a cycle) and 64 KiB are
@@ -52,9 +48,6 @@ typedef __attribute__((address_space(3))) void lvoid;
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-
-struct Yes { static constexpr bool v = true; };
-struct No { static constexpr bool v = false; };
 
 constexpr int kThreads = 256;
 
@@ -110,9 +103,19 @@ __device__ __forceinline__ void tile_of(int na, int nb, int& ta, int& tb) {
   tb = grp * G + (in - ta * gb);
 }
 
+// s_waitcnt with a count for one counter and the others left alone (vmcnt in
+// bits 0-3 and 14-15, expcnt in 4-6, lgkmcnt in 8-11).  As a builtin, so that
+// the compiler's own waits go on from it.
 template <int N> __device__ __forceinline__ void vm_wait() {
   static_assert(N >= 0 && N < 64, "vmcnt field");
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | 0x0f70 | (N >> 4) << 14);
+  asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void lds_read_wait() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);
+  asm volatile("" ::: "memory");
 }
 __device__ __forceinline__ void barrier_raw() {
   asm volatile("" ::: "memory");
@@ -137,7 +140,6 @@ struct Tile {
   static constexpr int kMuls = FA * FB;
   static_assert(KS == 128 || KS == 64, "image row");
   static_assert(!SPLIT || (FA % 2 == 0 && JA % 2 == 0), "both halves in whole fragments and loads");
-  static_assert(kDepths % 2 == 0, "fragment buffers alternate by depth");
   typedef typename E::frag frag;
   typedef typename E::acc32 acc_t;
 
@@ -175,43 +177,50 @@ struct Tile {
     const char* pa1 = p.a[1] + (int64_t)a0 * p.lda;
     const char* pb = p.b + (int64_t)b0 * p.ldb;
     const int64_t kbytes = p.kbytes;
+    // the operands' tiles as buffers: row offsets in a vector register, K in a scalar one
+    const auto ra0 = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(pa0), 0, -1, 0x27000);
+    const auto ra1 = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(pa1), 0, -1, 0x27000);
+    const auto rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(pb), 0, -1, 0x27000);
+    const auto rz = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint32_t*>(kZero16), 0, sizeof(kZero16), 0x27000);
 
     // load number j of step kt into the image at byte `at`; `tail`: the step may
-    // run past the end of K, where both sides read zeros
+    // run past the end of K, where both sides read zeros (one instruction more
+    // in flight, so that a wait by count is only longer).  Buffer loads: for a
+    // load through a global address the compiler, which cannot tell it from one
+    // that may reach LDS, waits for ALL fragment reads wherever it has to wait
+    // for one.
     auto load_one = [&](int kt, int at, int j, auto tail) {
-      char* img = lds + at + wave * 1024 + j * 4096;
-      const int64_t ko = (int64_t)kt * KS;
-      const bool is_a = j < JA;
-      // (the empty asm keeps the offset a 32-bit register next to its use, so
-      // that the address is scalar base + 32-bit offset and needs no VALU)
-      uint32_t& v = is_a ? va[is_a ? j : 0] : vb[is_a ? 0 : j - JA];
-      asm volatile("" : "+v"(v));
-      const char* s = (is_a ? (SPLIT && j >= JA / 2 ? pa1 : pa0) : pb) + ko + v;
-      if (decltype(tail)::v) s = ko + piece < kbytes ? s : reinterpret_cast<const char*>(kZero16);
-      __builtin_amdgcn_global_load_lds((gvoid*)s, (lvoid*)img, 16, 0, 0);
+      lvoid* img = (lvoid*)(lds + at + wave * 1024 + j * 4096);
+      const bool is_a = j < JA, upper = SPLIT && j >= JA / 2;
+      const auto r = is_a ? (upper ? ra1 : ra0) : rb;
+      const uint32_t v = is_a ? va[is_a ? j : 0] : vb[is_a ? 0 : j - JA];
+      if (!decltype(tail)::v || (int64_t)kt * KS + piece < kbytes)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, img, 16, v, kt * KS, 0, 0);
+      else
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rz, img, 16, 0, 0, 0, 0);
     };
     auto load = [&](int kt, int at) {
 #pragma unroll
-      for (int j = 0; j < kLoads; ++j) load_one(kt, at, j, Yes{});
+      for (int j = 0; j < kLoads; ++j) load_one(kt, at, j, ActK<1>{});
     };
 
     // ---- fragment reads: piece 2 d + g of depth d sits in slot (2 d + g) ^ swz(row) ----
     const int rho = 16 * ((r32 >> 2) & 1) + 4 * (r32 >> 3) + (r32 & 3);
     const int fa_at = (wa * (SPLIT ? RA / 4 : RA / 2) + rho) * KS + ((g ^ swz(rho)) << 4);
     const int fb_at = (RA + wb * (RB / 2) + r32) * KS + ((g ^ swz(r32)) << 4);
-    frag fa[2][FA], fb[2][FB];
+    frag fa[kDepths][FA], fb[kDepths][FB];
     // fragment t of the FB + FA of depth d
     auto read_one = [&](int at, int d, int t) {
       if (t < FB) {
-        fb[d & 1][t] = *reinterpret_cast<const frag*>(lds + at + (fb_at ^ (d << 5)) + t * 32 * KS);
+        fb[d][t] = *reinterpret_cast<const frag*>(lds + at + (fb_at ^ (d << 5)) + t * 32 * KS);
       } else {
         const int i = t - FB;
         const int row = SPLIT ? (i >= FA / 2 ? RA / 2 : 0) + 32 * (i % (FA / 2)) : 32 * i;
-        fa[d & 1][i] = *reinterpret_cast<const frag*>(lds + at + (fa_at ^ (d << 5)) + row * KS);
+        fa[d][i] = *reinterpret_cast<const frag*>(lds + at + (fa_at ^ (d << 5)) + row * KS);
       }
     };
     auto mul_one = [&](int d, int q) {
-      acc[q / FB][q % FB] = E::mul32(fa[d & 1][q / FB], fb[d & 1][q % FB], acc[q / FB][q % FB]);
+      acc[q / FB][q % FB] = E::mul32(fa[d][q / FB], fb[d][q % FB], acc[q / FB][q % FB]);
     };
 
 #pragma unroll
@@ -230,42 +239,66 @@ struct Tile {
 #pragma unroll
     for (int t = 0; t < kReads; ++t) read_one(at, 0, t);
 
-    // depth d of image `at`, the reads of the next depth (of image `next`) and
-    // with `ld` the loads of step kt dealt out among its MFMAs: the source
-    // order, which the sched_barriers keep, is the schedule
-    auto depth = [&](int d, int next, auto ld, int kt) {
-#pragma unroll
-      for (int q = 0; q < kMuls; ++q) {
-        if (decltype(ld)::v) {
-#pragma unroll
-          for (int t = q * kLoads / kMuls; t < (q + 1) * kLoads / kMuls; ++t) load_one(kt, at, t, No{});
-        }
-#pragma unroll
-        for (int t = q * kReads / kMuls; t < (q + 1) * kReads / kMuls; ++t) read_one(next, (d + 1) % kDepths, t);
-        mul_one(d, q);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+    // One step: kSlots MFMAs, with everything else dealt out among them by hand
+    // (the source order, which the sched_barriers keep, is the schedule):
+    //   first 3/8    reads of depths 1 ..
+    //   half         barrier: every wave has read the image
+    //   second half  loads of step kt + NST into its place
+    //   7/8          wait for step kt + 1, barrier; then reads of its depth 0
+    // Reads are bunched and loads spread because the two images must cover a
+    // load's way to memory: an image is free for half a step more than if its
+    // reads took the whole step, and a load every 64 cycles and wave is what the
+    // address unit takes (16 cycles each): 16 in a quarter of the step stalled
+    // the MFMAs behind them.
+    constexpr int S = kDepths * kMuls, kB1 = S / 2, kB2 = S * 7 / 8, kR = (kDepths - 1) * kReads, kRS = (S * 3 + 7) / 8;
+    constexpr int kBefore = (kB2 - kB1) * kLoads / (S - kB1);  // loads issued before the second wait
+    auto mul_slot = [&](int s) {
+      mul_one(s / kMuls, s % kMuls);
+      __builtin_amdgcn_sched_barrier(0);
     };
-    auto step = [&](int kt, auto full) {
+    auto read_slot = [&](int s) {
 #pragma unroll
-      for (int d = 0; d + 1 < kDepths; ++d) depth(d, at, No{}, 0);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (decltype(full)::v || kt + NST <= k1) vm_wait<(NST - 2) * kLoads>(); else vm_wait<0>();
-      barrier_raw();
-      if (!decltype(full)::v && kt + NST < k1) load(kt + NST, at);
+      for (int t = s * kR / kRS; t < (s + 1) * kR / kRS; ++t) read_one(at, 1 + t / kReads, t % kReads);
+    };
+    // mode 0: a load that lies wholly inside K; 1: one that may run past its
+    // end; 2: no load
+    auto step = [&](int kt, auto mode) {
+      constexpr int kMode = decltype(mode)::v;
       const int next = at + kImage == kLds ? 0 : at + kImage;
-      depth(kDepths - 1, next, full, kt + NST);
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        if (s < kRS) read_slot(s);
+        if (s == kB1) {
+          lds_read_wait();
+          barrier_raw();
+        }
+        if (s == kB2) {
+          if (kMode < 2) vm_wait<(NST - 2) * kLoads + kBefore>(); else vm_wait<0>();
+          barrier_raw();
+        }
+        if (kMode < 2 && s >= kB1) {
+#pragma unroll
+          for (int t = (s - kB1) * kLoads / (S - kB1); t < (s - kB1 + 1) * kLoads / (S - kB1); ++t)
+            load_one(kt + NST, at, t, ActK<kMode>{});
+        }
+        if (s >= kB2) {
+#pragma unroll
+          for (int t = (s - kB2) * kReads / (S - kB2); t < (s - kB2 + 1) * kReads / (S - kB2); ++t) read_one(next, 0, t);
+        }
+        mul_slot(s);
+      }
       at = next;
     };
     int kt = k0;
-    // steps whose load lies wholly inside K
-    const int kfull = min(k1, (int)(kbytes / KS)) - NST;
-    for (; kt < kfull; ++kt) step(kt, Yes{});
-    for (; kt + 1 < k1; ++kt) step(kt, No{});
+    const int kfull = min(k1, (int)(kbytes / KS)) - NST;  // steps whose load lies wholly inside K
+    for (; kt < kfull; ++kt) step(kt, ActK<0>{});
+    for (; kt + NST < k1; ++kt) step(kt, ActK<1>{});
+    for (; kt + 1 < k1; ++kt) step(kt, ActK<2>{});
 #pragma unroll
-    for (int d = 0; d + 1 < kDepths; ++d) depth(d, at, No{}, 0);
-#pragma unroll
-    for (int q = 0; q < kMuls; ++q) mul_one(kDepths - 1, q);
+    for (int s = 0; s < S; ++s) {
+      if (s < kRS) read_slot(s);
+      mul_slot(s);
+    }
   }
 };
 
