@@ -345,10 +345,18 @@ struct RowStore {
         if (m < M && n < N) *reinterpret_cast<f32x4*>(out + (int64_t)m * N + n) = v;
       }
     } else {
-      for (int e = lane; e < 32 * 32 * NF; e += 64) {
-        const int row = e / (32 * NF), c = e % (32 * NF), m = m0 + row, n = n0 + c;
-        const TO v = *reinterpret_cast<const TO*>(lds + at(row, c / kVec) + (c % kVec) * (int)sizeof(TO));
-        if (m < M && n < N) out[(int64_t)m * N + n] = v;
+      // rows of any length: single elements, 64 (or two rows of 32) a store
+      constexpr int kCols = 32 * NF, kLanes = kCols < 64 ? kCols : 64;
+      const int c = lane % kLanes, r0 = lane / kLanes;
+      TO* q = out + (int64_t)(m0 + r0) * N + n0 + c;
+#pragma unroll 8
+      for (int row = r0; row < 32; row += 64 / kLanes) {
+#pragma unroll
+        for (int k = 0; k < kCols; k += kLanes) {
+          const TO v = *reinterpret_cast<const TO*>(lds + at(row, (c + k) / kVec) + ((c + k) % kVec) * (int)sizeof(TO));
+          if (m0 + row < M && n0 + c + k < N) q[k] = v;
+        }
+        q += (int64_t)(64 / kLanes) * N;
       }
     }
   }

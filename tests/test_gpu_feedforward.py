@@ -426,6 +426,7 @@ def test_distill_kl_masks(cuda, N):
     z[6, : N // 2] = -math.inf
     ti[6] = N - 1 - torch.arange(6, device=cuda)
     z[7, : N // 2] = low
+    z[3] = low  # nothing but the lowest value: even odds
     ti[7] = N - 1 - torch.arange(6, device=cuda)
     tv[8, 3] = float("nan")
     ti[8, 3] = -1  # a NaN that is not there
@@ -434,6 +435,31 @@ def test_distill_kl_masks(cuda, N):
         assert loss[row].item() == 0 and not dz[row].any(), row
     tv[8, 3] = 0.0
     distill_check(z[3:], tv[3:], ti[3:], 1.5, 1.0, dz[3:], loss[3:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shift", [-3e4, 1e6])
+def test_distill_kl_logits_far_from_zero(cuda, shift):
+    """A row's logits count by their differences alone (here exact: multiples of 1/4 below 2^24 / 4)."""
+    g = gen(8, cuda)
+    z = torch.randint(-40, 40, (5, 3001), device=cuda, generator=g) / 4.0
+    tv = torch.randint(-40, 40, (5, 7), device=cuda, generator=g) / 4.0
+    ti = torch.randint(0, 3001, (5, 7), device=cuda, generator=g)
+    a, b = ops.distill_kl(z, tv, ti, temperature=2.0), ops.distill_kl(z + shift, tv + shift, ti, temperature=2.0)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,pad", [(1000, 3), (20000, 5), (40001, 8), (150000, 1)])
+def test_distill_kl_strided_logits(cuda, N, pad):
+    """Rows of a wider matrix, another pitch than the gradient's and a start that is not aligned."""
+    g = gen(8, cuda)
+    z, tv, ti = distill_case(g, 3, N + pad, 9, torch.bfloat16)
+    ti = ti.clamp(max=N - 1)
+    view = z[:, pad // 2 : pad // 2 + N]
+    a, b = ops.distill_kl(view, tv, ti), ops.distill_kl(view.contiguous(), tv, ti)
+    distill_check(view, tv, ti, 1.0, 1.0, a[0], a[1])
+    distill_check(view, tv, ti, 1.0, 1.0, b[0], b[1])
 
 
 @pytest.mark.gpu
