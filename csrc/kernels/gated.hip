@@ -105,6 +105,19 @@ __global__ void __launch_bounds__(64 * NW) gated_rows_kernel(GatedParams p, Oper
   });
 }
 
+// outputs a workgroup (gate and projection at once), workgroups a CU, us a step:
+// 1024^3 256 workgroups of the first form 7.8 us, of the second (128) 10.3;
+// 3000 x 512 x 4096 37.0 / 31.3 / 43.9 us; 1024 x 4096 x 4096 84 / 62 / 58 / 79;
+// 4096^3 343 / 251 / 233 / 206
+constexpr tile::Form kForms[] = {{64, 64, 2, 0.27f, 0.67f}, {64, 128, 2, 0.46f, 0.97f}, {128, 128, 1, 0.9f, 0.9f},
+                                 {128, 256, 1, 1.61f, 1.61f}};
+
+template <int FA, int FB, int NST, int WPE, int ACT>
+void launch_tiles(const GatedParams& p, const Operands& o, hipStream_t s) {
+  const dim3 grid((unsigned)(cdiv(p.F, 32 * FA) * cdiv(p.M, 64 * FB)));
+  hipLaunchKernelGGL((gated_tile_kernel<FA, FB, 128, NST, WPE, ACT>), grid, dim3(tile::kThreads), 0, s, p, o);
+}
+
 }  // namespace
 
 void gated_forward(const GatedParams& p, hipStream_t s) {
@@ -118,20 +131,27 @@ void gated_forward(const GatedParams& p, hipStream_t s) {
   MCC_CHECK((p.gate == nullptr) == (p.up == nullptr), "gated_linear: gate and up go together");
   if (p.M == 0) return;
   const Operands o = operands(p);
-  if (p.M <= 64) {
-    const dim3 grid((unsigned)cdiv(p.F, 16), 1);
-    if (p.M <= 16) hipLaunchKernelGGL((gated_rows_kernel<1, 4, 4>), grid, dim3(256), 0, s, p, o);
-    else if (p.M <= 32) hipLaunchKernelGGL((gated_rows_kernel<2, 2, 4>), grid, dim3(256), 0, s, p, o);
-    else hipLaunchKernelGGL((gated_rows_kernel<4, 1, 4>), grid, dim3(256), 0, s, p, o);
-  } else if ((int64_t)cdiv(p.F, 128) * cdiv(p.M, 256) >= 256) {
-    const dim3 grid((unsigned)(cdiv(p.F, 128) * cdiv(p.M, 256)));
-    with_gate(p.act, [&](auto k) {
-      hipLaunchKernelGGL((gated_tile_kernel<4, 4, 128, 2, 1, decltype(k)::v>), grid, dim3(tile::kThreads), 0, s, p, o);
-    });
+  // up to 32 rows the weights' way from memory counts, which many workgroups
+  // that stream share best; above, whatever the measured step times say
+  const int64_t n1 = (int64_t)cdiv(p.F, 16) * cdiv(p.M, 16), n2 = (int64_t)cdiv(p.F, 16) * cdiv(p.M, 32);
+  const int form = tile::best_form(kForms, p.F, p.M);
+  const float tiles = tile::step_us(kForms[form], tile::workgroups(kForms[form], p.F, p.M));
+  const float rows1 = tile::few_rows_us(true, 1, n1);
+  if (p.M <= 16 || (p.M <= 32 ? rows1 <= tile::few_rows_us(true, 2, n2) : rows1 < tiles)) {
+    const dim3 grid((unsigned)cdiv(p.F, 16), (unsigned)cdiv(p.M, 16));
+    if (o.kbytes >= 4096) hipLaunchKernelGGL((gated_rows_kernel<1, 4, 8>), grid, dim3(512), 0, s, p, o);
+    else hipLaunchKernelGGL((gated_rows_kernel<1, 4, 4>), grid, dim3(256), 0, s, p, o);
+  } else if (p.M <= 32) {
+    hipLaunchKernelGGL((gated_rows_kernel<2, 2, 4>), dim3((unsigned)cdiv(p.F, 16)), dim3(256), 0, s, p, o);
   } else {
-    const dim3 grid((unsigned)(cdiv(p.F, 64) * cdiv(p.M, 128)));
     with_gate(p.act, [&](auto k) {
-      hipLaunchKernelGGL((gated_tile_kernel<2, 2, 128, 2, 2, decltype(k)::v>), grid, dim3(tile::kThreads), 0, s, p, o);
+      constexpr int A = decltype(k)::v;
+      switch (form) {
+        case 0: launch_tiles<2, 1, 3, 2, A>(p, o, s); break;
+        case 1: launch_tiles<2, 2, 2, 2, A>(p, o, s); break;
+        case 2: launch_tiles<4, 2, 3, 1, A>(p, o, s); break;
+        default: launch_tiles<4, 4, 2, 1, A>(p, o, s); break;
+      }
     });
   }
   MCC_CHECK(hipGetLastError() == hipSuccess, "gated_linear: launch failed");

@@ -182,31 +182,50 @@ __global__ void __launch_bounds__(256) sum_partials_kernel(const float* part, in
   }
 }
 
-// K splits of a product that has few tiles: enough for two workgroups per CU, at
-// least 8 steps each
-int splits_of(int64_t tiles, int64_t steps) {
-  if (tiles >= 256 || steps < 16) return 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>((512 + tiles - 1) / tiles, steps / 8));
+// outputs a workgroup, workgroups a CU, us a step (tile_gemm.h: Form)
+constexpr tile::Form kForms[] = {{64, 64, 2, 0.22f, 0.5f}, {128, 64, 2, 0.33f, 0.67f}, {128, 128, 2, 0.46f, 0.97f},
+                                 {256, 256, 1, 1.55f, 1.55f}};
+// How a product is done: its form, and into how many sums over K it is split
+// where it has few tiles (1024 x 777 outputs, K = 5472: 37.0 us in 56 tiles of
+// 128 x 128, 15.5 in 4 sums of them and 5 to add these up; 21.8 in 208 tiles of
+// 64 x 64)
+struct How {
+  int form, S;
+};
+How how_of(int64_t arows, int64_t brows, int64_t kbytes) {
+  const int64_t steps = (kbytes + 127) / 128;
+  How best{0, 1};
+  float least = 1e30f;
+  for (int f = 0; f < 4; ++f) {
+    const int64_t n = tile::workgroups(kForms[f], arows, brows);
+    // (the largest form has no split: it is for products that fill the chip)
+    for (int S = 1; S <= (f == 3 ? 1 : 16) && steps / S >= 4; S *= 2) {
+      const float join = S == 1 ? 0.f : 4.f + (float)S * arows * brows * 8.f / 4e6f;
+      const float us = tile::step_us(kForms[f], n * S) * (float)((steps + S - 1) / S) + join;
+      if (us < least) {
+        least = us;
+        best = {f, S};
+      }
+    }
+    if (steps < 4 && tile::step_us(kForms[f], n) < least) {
+      least = tile::step_us(kForms[f], n);
+      best = {f, 1};
+    }
+  }
+  return best;
 }
 
 struct Plan {
   int Fp, Mp;
-  int sx;          // K splits of dX
-  int sw;          // ... of dW
+  How x, w;  // dX and dW
   int64_t dgu, dgut, wt, xt, part, total;  // byte offsets
 };
-bool big_tiles(int64_t rows, int64_t cols) { return cdiv((int)cols, 256) * (int64_t)cdiv((int)rows, 256) >= 256; }
-int splits(int64_t rows, int64_t cols, int64_t kbytes) {
-  if (big_tiles(rows, cols)) return 1;
-  return splits_of((int64_t)cdiv((int)cols, 128) * cdiv((int)rows, 128), (kbytes + 127) / 128);
-}
-
 Plan plan_of(int M, int D, int F) {
   Plan q;
   q.Fp = (int)round_up(F, 8);
   q.Mp = (int)round_up(M, 8);
-  q.sx = splits(M, D, 4 * (int64_t)q.Fp);
-  q.sw = splits(2 * (int64_t)F, D, 2 * (int64_t)q.Mp);
+  q.x = how_of(D, M, 4 * (int64_t)q.Fp);
+  q.w = how_of(D, 2 * (int64_t)F, 2 * (int64_t)q.Mp);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t o = at;
@@ -217,14 +236,25 @@ Plan plan_of(int M, int D, int F) {
   q.dgut = take(2 * 2 * (int64_t)F * q.Mp);
   q.wt = take(2 * (int64_t)D * 2 * q.Fp);
   q.xt = take(2 * (int64_t)D * q.Mp);
-  const int64_t px = q.sx > 1 ? 4 * q.sx * (int64_t)M * D : 0, pw = q.sw > 1 ? 4 * q.sw * 2 * (int64_t)F * D : 0;
+  const int64_t px = q.x.S > 1 ? 4 * q.x.S * (int64_t)M * D : 0, pw = q.w.S > 1 ? 4 * q.w.S * 2 * (int64_t)F * D : 0;
   q.part = take(std::max(px, pw));
   q.total = at;
   return q;
 }
 
+template <int FA, int FB, int NST, int WPE, class TO>
+void launch_tiles(const Operands& o, TO* out, int steps, int S, hipStream_t s) {
+  const dim3 grid((unsigned)(cdiv(o.arows, 64 * FA) * cdiv(o.brows, 64 * FB)), (unsigned)S);
+  hipLaunchKernelGGL((tile_store_kernel<FA, FB, 128, NST, WPE, TO>), grid, dim3(tile::kThreads), 0, s, o, out, steps);
+}
+template <class TO> void launch_form(int form, const Operands& o, TO* out, int steps, int S, hipStream_t s) {
+  if (form == 0) launch_tiles<1, 1, 4, 2, TO>(o, out, steps, S, s);
+  else if (form == 1) launch_tiles<2, 1, 3, 2, TO>(o, out, steps, S, s);
+  else launch_tiles<2, 2, 2, 2, TO>(o, out, steps, S, s);
+}
+
 // out [brows][arows] = B A^T
-void product(const char* a, int arows, const char* b, int brows, int64_t kbytes, bf16* out, float* part, int S,
+void product(const char* a, int arows, const char* b, int brows, int64_t kbytes, bf16* out, float* part, How how,
              hipStream_t s) {
   Operands o;
   o.a[0] = o.a[1] = a;
@@ -235,22 +265,16 @@ void product(const char* a, int arows, const char* b, int brows, int64_t kbytes,
   o.kbytes = kbytes;
   MCC_CHECK(kbytes <= (1 << 23), "gated_linear_bwd: row too long");
   const int steps = (int)((kbytes + 127) / 128);
-  if (big_tiles(brows, arows)) {
-    const dim3 grid((unsigned)(cdiv(arows, 256) * cdiv(brows, 256)));
-    hipLaunchKernelGGL((tile_store_kernel<4, 4, 128, 2, 1, bf16>), grid, dim3(tile::kThreads), 0, s, o, out, steps);
-    return;
+  const int per = cdiv(steps, how.S), S = cdiv(steps, per);
+  if (how.form == 3) {
+    launch_tiles<4, 4, 2, 1, bf16>(o, out, steps, 1, s);
+  } else if (S == 1) {
+    launch_form<bf16>(how.form, o, out, steps, 1, s);
+  } else {
+    launch_form<float>(how.form, o, part, per, S, s);
+    const int64_t n = (int64_t)arows * brows;
+    hipLaunchKernelGGL(sum_partials_kernel, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, s, part, n, S, out);
   }
-  const unsigned tiles = (unsigned)(cdiv(arows, 128) * cdiv(brows, 128));
-  if (S == 1) {
-    hipLaunchKernelGGL((tile_store_kernel<2, 2, 128, 2, 2, bf16>), dim3(tiles), dim3(tile::kThreads), 0, s, o, out, steps);
-    return;
-  }
-  const int per = cdiv(steps, S);
-  S = cdiv(steps, per);
-  hipLaunchKernelGGL((tile_store_kernel<2, 2, 128, 2, 2, float>), dim3(tiles, (unsigned)S), dim3(tile::kThreads), 0, s, o,
-                     part, per);
-  const int64_t n = (int64_t)arows * brows;
-  hipLaunchKernelGGL(sum_partials_kernel, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, s, part, n, S, out);
 }
 
 void transpose(const void* in, int64_t ld, int rows, int cols, bf16* out, int64_t ldo, int rows_pad, hipStream_t s) {
@@ -289,9 +313,9 @@ void gated_backward(const GatedBwdParams& p, hipStream_t s) {
   transpose(p.wu, p.ldw, p.F, p.D, wt + q.Fp, 2 * q.Fp, q.Fp, s);
   transpose(p.x, p.ldx, p.M, p.D, xt, q.Mp, q.Mp, s);
   product(reinterpret_cast<const char*>(wt), p.D, reinterpret_cast<const char*>(dgu), p.M, 4 * (int64_t)q.Fp,
-          static_cast<bf16*>(p.dx), part, q.sx, s);
+          static_cast<bf16*>(p.dx), part, q.x, s);
   product(reinterpret_cast<const char*>(xt), p.D, reinterpret_cast<const char*>(dgut), 2 * p.F, 2 * (int64_t)q.Mp,
-          static_cast<bf16*>(p.dw), part, q.sw, s);
+          static_cast<bf16*>(p.dw), part, q.w, s);
   MCC_CHECK(hipGetLastError() == hipSuccess, "gated_linear_bwd: launch failed");
 }
 

@@ -110,6 +110,13 @@ void launch_tiles(const LinearI8Params& p, const Operands& o, hipStream_t s) {
     hipLaunchKernelGGL((i8_tile_kernel<FA, FB, KS, NST, WPE, ACT_NONE, TO>), grid, dim3(tile::kThreads), 0, s, p, o);
 }
 
+// outputs a workgroup, workgroups a CU, us a step: 640 x 1000 x 4096 9.8 / 11.6 /
+// 16.1 / 37.6 us, 2048^3 16.8 / 15.2 / 13.1 / 25.3, 1024 x 4096 x 4096 29.4 / 25.7
+// / 22.6 / 40.3, 4096^3 117 / 91 / 68 / 60 (and 256 x 128 tiles, which win
+// nowhere, 23.0, 17.7, 29.5, 69)
+constexpr tile::Form kForms[] = {{64, 64, 2, 0.21f, 0.45f}, {128, 64, 2, 0.28f, 0.69f}, {128, 128, 2, 0.6f, 1.03f},
+                                 {256, 256, 1, 1.75f, 1.75f}};
+
 template <class TO> void launch(const LinearI8Params& p, hipStream_t s) {
   Operands o;
   o.a[0] = o.a[1] = static_cast<const char*>(p.w);
@@ -119,17 +126,25 @@ template <class TO> void launch(const LinearI8Params& p, hipStream_t s) {
   o.arows = p.N;
   o.brows = p.M;
   o.kbytes = round_up(p.K, 16);
-  if (p.M <= 64) {
-    const dim3 grid((unsigned)cdiv(p.N, 16), 1);
-    if (p.M <= 16) hipLaunchKernelGGL((i8_rows_kernel<1, 4, 4, TO>), grid, dim3(256), 0, s, p, o);
-    else if (p.M <= 32) hipLaunchKernelGGL((i8_rows_kernel<2, 2, 4, TO>), grid, dim3(256), 0, s, p, o);
-    else hipLaunchKernelGGL((i8_rows_kernel<4, 1, 4, TO>), grid, dim3(256), 0, s, p, o);
-  } else if ((int64_t)cdiv(p.N, 256) * cdiv(p.M, 256) >= 256) {
-    launch_tiles<4, 4, 128, 2, 1, TO>(p, o, s);
-  } else if ((int64_t)cdiv(p.N, 128) * cdiv(p.M, 128) >= 256) {
-    launch_tiles<2, 2, 128, 2, 2, TO>(p, o, s);
+  // up to 32 rows the weights' way from memory counts, which many workgroups
+  // that stream share best; above, whatever the measured step times say
+  const int64_t n1 = (int64_t)cdiv(p.N, 16) * cdiv(p.M, 16), n2 = (int64_t)cdiv(p.N, 16) * cdiv(p.M, 32);
+  const int form = tile::best_form(kForms, p.N, p.M);
+  const float tiles = tile::step_us(kForms[form], tile::workgroups(kForms[form], p.N, p.M));
+  const float rows1 = tile::few_rows_us(false, 1, n1);
+  if (p.M <= 16 || (p.M <= 32 ? rows1 <= tile::few_rows_us(false, 2, n2) : rows1 < tiles)) {
+    const dim3 grid((unsigned)cdiv(p.N, 16), (unsigned)cdiv(p.M, 16));
+    if (o.kbytes >= 4096) hipLaunchKernelGGL((i8_rows_kernel<1, 4, 8, TO>), grid, dim3(512), 0, s, p, o);
+    else hipLaunchKernelGGL((i8_rows_kernel<1, 4, 4, TO>), grid, dim3(256), 0, s, p, o);
+  } else if (p.M <= 32) {
+    hipLaunchKernelGGL((i8_rows_kernel<2, 2, 4, TO>), dim3((unsigned)cdiv(p.N, 16)), dim3(256), 0, s, p, o);
   } else {
-    launch_tiles<1, 1, 128, 4, 2, TO>(p, o, s);
+    switch (form) {
+      case 0: launch_tiles<1, 1, 128, 4, 2, TO>(p, o, s); break;
+      case 1: launch_tiles<2, 1, 128, 3, 2, TO>(p, o, s); break;
+      case 2: launch_tiles<2, 2, 128, 2, 2, TO>(p, o, s); break;
+      default: launch_tiles<4, 4, 128, 2, 1, TO>(p, o, s); break;
+    }
   }
   MCC_CHECK(hipGetLastError() == hipSuccess, "linear_i8: launch failed");
 }

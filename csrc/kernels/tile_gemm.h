@@ -362,6 +362,31 @@ struct RowStore {
   }
 };
 
+// ---- choice of a tile (host) ----
+// A form of a product: workgroups of `rows_a` x `rows_b` outputs, `per_cu` of
+// them to a CU, and what a step of 128 bytes of K takes, measured in us: `one`
+// while a CU holds one workgroup, `full` while it holds all `per_cu`.
+struct Form {
+  int rows_a, rows_b, per_cu;
+  float one, full;
+};
+constexpr int kCus = 256;
+inline int64_t workgroups(const Form& f, int64_t arows, int64_t brows) {
+  return (arows + f.rows_a - 1) / f.rows_a * ((brows + f.rows_b - 1) / f.rows_b);
+}
+// us per step of n workgroups: whole rounds of the chip, then what is left
+inline float step_us(const Form& f, int64_t n) {
+  const int64_t slots = (int64_t)kCus * f.per_cu, rest = n % slots;
+  return n / slots * f.full + (rest == 0 ? 0.f : rest <= kCus ? f.one : f.full);
+}
+// the form that takes least
+template <int N> inline int best_form(const Form (&f)[N], int64_t arows, int64_t brows) {
+  int best = 0;
+  for (int i = 1; i < N; ++i)
+    if (step_us(f[i], workgroups(f[i], arows, brows)) < step_us(f[best], workgroups(f[best], arows, brows))) best = i;
+  return best;
+}
+
 }  // namespace tile
 }  // namespace gpu
 }  // namespace mcc

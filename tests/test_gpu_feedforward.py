@@ -81,7 +81,9 @@ def gated_check(x, wg, wu, act, out, save):
 
 GATED = [(1, 64, 16), (1, 8, 1), (1, 1, 3), (2, 136, 70), (16, 512, 100), (17, 264, 33), (32, 1000, 64), (33, 72, 257),
          (64, 4104, 48), (65, 64, 64), (66, 1, 5), (100, 333, 129), (128, 128, 64), (129, 192, 65), (300, 200, 515),
-         (1000, 520, 130), (4097, 64, 1030), (2050, 136, 4232)]
+         (1000, 520, 130), (4097, 64, 1030), (2050, 136, 4232),
+         # the forms that the sizes above do not reach: two groups of 16 rows, 128 x 128 and 128 x 256 tiles
+         (24, 72, 4500), (31, 1032, 4099), (1030, 72, 2063), (1024, 200, 2048), (4090, 72, 4090), (4096, 136, 4096)]
 
 
 @pytest.mark.gpu
@@ -133,7 +135,8 @@ def i8_check(x, sx, w, sw, b, act, y):
 
 
 I8 = [(1, 16, 16), (1, 1, 1), (3, 5, 7), (16, 100, 4096), (17, 33, 1000), (33, 64, 144), (64, 1000, 272), (65, 64, 128),
-      (128, 128, 640), (130, 70, 130), (640, 1000, 512), (1030, 4100, 176), (4100, 4360, 144), (70, 17, 20000)]
+      (128, 128, 640), (130, 70, 130), (640, 1000, 512), (1030, 4100, 176), (4100, 4360, 144), (70, 17, 20000),
+      (20, 6000, 500), (32, 4097, 4112), (1500, 1999, 400), (4090, 4090, 272), (4096, 4096, 100)]
 
 
 @pytest.mark.gpu
@@ -197,7 +200,12 @@ def gated_bwd_case(g, M, D, F, std=1.0):
 
 GATED_BWD = [(1, 64, 16), (1, 1, 1), (2, 136, 70), (3, 9, 1), (16, 512, 100), (17, 264, 33), (33, 72, 257), (64, 4104, 48),
              (64, 128, 3000), (65, 64, 64), (66, 1, 5), (100, 333, 129), (128, 128, 64), (129, 192, 65), (300, 200, 515),
-             (1000, 520, 130), (4100, 64, 1030), (700, 4360, 4200)]
+             (1000, 520, 130), (4100, 64, 1030), (700, 4360, 4200),
+             # every form and split of the two products
+             (2634, 8, 2330), (1797, 185, 1), (2073, 16, 10), (36, 141, 2829), (2763, 4656, 1), (2178, 2144, 1),
+             (33, 259, 2940), (34, 1808, 3272), (91, 10, 848), (55, 8, 1024), (33, 8, 2024), (129, 4208, 3876),
+             (66, 2096, 1296), (66, 1028, 1520), (33, 1035, 2904), (2144, 1170, 1), (193, 4136, 2339), (66, 4240, 2081),
+             (2078, 70, 1416), (67, 1048, 2845)]
 
 
 @pytest.mark.gpu
