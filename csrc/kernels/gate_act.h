@@ -9,11 +9,29 @@ namespace gpu {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// The normal distribution function and exp(-v^2 / 2), by the rational form of
+// Abramowitz and Stegun 7.1.26: erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2),
+// t = 1 / (1 + p x), off by at most 1.5e-7 for x >= 0; halved here, and for
+// v < 0 without a difference that would lose it.  A library erff took 8 us of
+// 23 at 777 x 1024 x 2736.
+__device__ __forceinline__ void normal(float v, float& cdf, float& bell) {
+  bell = __builtin_amdgcn_exp2f(-0.5f * kLog2e * v * v);
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, fabsf(v), 1.f));
+  const float half =
+      t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f), 0.5f * 1.421413741f),
+                       0.5f * -0.284496736f), 0.5f * 0.254829592f) * bell;
+  cdf = v < 0.f ? half : 1.f - half;
+}
+
 template <int A> __device__ __forceinline__ float gate_f(float v) {
   if constexpr (A == GATE_RELU) return v < 0.f ? 0.f : v;  // keeps a NaN
   if constexpr (A == GATE_TANH) return tanhf(v);
   if constexpr (A == GATE_SILU) return v / (1.f + __builtin_amdgcn_exp2f(-kLog2e * v));
-  if constexpr (A == GATE_GELU) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+  if constexpr (A == GATE_GELU) {
+    float cdf, bell;
+    normal(v, cdf, bell);
+    return v * cdf;
+  }
   return v;
 }
 
@@ -41,9 +59,10 @@ template <int A> __device__ __forceinline__ void gate_slope(float v, float& f, f
     f = v * s;
     d = s * (1.f + v * (1.f - s));
   } else if constexpr (A == GATE_GELU) {
-    const float c = 0.5f * (1.f + erff(v * 0.70710678118654752f));
-    f = v * c;
-    d = c + v * (0.39894228040143268f * __builtin_amdgcn_exp2f(-0.5f * kLog2e * v * v));
+    float cdf, bell;
+    normal(v, cdf, bell);
+    f = v * cdf;
+    d = fmaf(v, 0.39894228040143268f * bell, cdf);
   } else {
     f = v;
     d = 1.f;
