@@ -26,7 +26,7 @@ __device__ __forceinline__ void normal(float v, float& cdf, float& bell) {
 template <int A> __device__ __forceinline__ float gate_f(float v) {
   if constexpr (A == GATE_RELU) return v < 0.f ? 0.f : v;  // keeps a NaN
   if constexpr (A == GATE_TANH) return tanhf(v);
-  if constexpr (A == GATE_SILU) return v / (1.f + __builtin_amdgcn_exp2f(-kLog2e * v));
+  if constexpr (A == GATE_SILU) return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * v));
   if constexpr (A == GATE_GELU) {
     float cdf, bell;
     normal(v, cdf, bell);
@@ -55,7 +55,7 @@ template <int A> __device__ __forceinline__ void gate_slope(float v, float& f, f
     f = tanhf(v);
     d = 1.f - f * f;
   } else if constexpr (A == GATE_SILU) {
-    const float s = 1.f / (1.f + __builtin_amdgcn_exp2f(-kLog2e * v));
+    const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * v));
     f = v * s;
     d = s * (1.f + v * (1.f - s));
   } else if constexpr (A == GATE_GELU) {

@@ -1,18 +1,20 @@
 // Backward pass of the gated feed-forward block (feedforward.h: GatedBwdParams).
 //
-//   1. gated_grad: dG, dU from dH, G, U, written twice: [M][2 Fp] for dX (whose
-//      K runs along F) and transposed [2 F][Mp] for dW (whose K runs along M).
-//   2. dX [M][D] = dGU [M][2 Fp] * WT [D][2 Fp]^T,  WT = both weights transposed
+//   1. gated_prepare: dG, dU from dH, G, U, written twice: [M][2 Fp] for dX
+//      (whose K runs along F) and transposed [2 F][Mp] for dW (whose K runs
+//      along M); X transposed, and the weights unless 2b. follows
+//   2a. dX [M][D] = dGU [M][2 Fp] * WT [D][2 Fp]^T, or
+//   2b. up to 128 rows dX from the weights as they are (gated_dx_rows_kernel)
 //   3. dW [2F][D] = dGUT [2F][Mp] * XT [D][Mp]^T
 //
 // Transposes instead of operands read across their rows: every product is then
 // the one tile loop of tile_gemm.h, and the transposes move M D + 2 F D + 2 M F
-// elements once more.  At 8192 x 4096 x 12288 that is 0.9 GB beside
-// 3.3 TFLOP.  Up to 64 rows the weights' bytes are the whole cost: dX then reads
-// the weights as they are (gated_dx_rows).
+// elements once more.  At 8192 x 4096 x 12288 that is 0.9 GB (0.4 ms with dG and
+// dU themselves) beside 3.3 TFLOP (2.4 ms).  For few rows the weights' bytes are
+// the whole cost, and 2b. reads them once.
 //
 // dG and dU are rounded to bf16, the operand type of the matrix unit: an
-// independent error of 2^-9 rms per term, so 2^-9 rms of the sum as well.
+// independent error of at most 2^-8 per term, so no more of the sum's terms.
 #include "feedforward.h"
 #include "gate_act.h"
 #include "kernels.h"
@@ -38,15 +40,43 @@ __device__ __forceinline__ bf16x8 cvt8(const float (&v)[8]) {
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// 8 elements from column c on of a row with n columns, zeros past its end.
-// wide: the row starts on 16 bytes and n is a multiple of 8.
-__device__ __forceinline__ bf16x8 get8(const bf16* row, int c, int n, bool wide) {
-  if (wide) {
-    if (c + 8 <= n) return load8(row + c);
-  }
-  bf16x8 v;
+// A matrix to be read in runs of 8 columns from any 2-byte address and pitch.
+struct Source {
+  const bf16* p;
+  int64_t ld, size;  // pitch, and elements from p to the last one
+  int rows, cols;
+};
+Source source(const void* p, int64_t ld, int rows, int cols) {
+  return Source{static_cast<const bf16*>(p), ld, (rows - 1) * ld + cols, rows, cols};
+}
+// columns c .. c+7 of row r, zeros where there are none.  A run that does not
+// start on 16 bytes is cut out of the two aligned pieces that hold it, where
+// both lie inside the matrix.
+__device__ __forceinline__ bf16x8 get8(const Source& m, int r, int c) {
+  bf16x8 v = {};
+  if (r >= m.rows || c >= m.cols) return v;
+  const int64_t at = r * m.ld + c;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(m.p + at);
+  const int off = (int)(a & 15) / 2;
+  if (off == 0 && at + 8 <= m.size) {
+    v = load8(m.p + at);
+  } else if (at - off >= 0 && at - off + 16 <= m.size) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    typedef uint32_t u8 __attribute__((ext_vector_type(8)));
+    const u4 lo = *reinterpret_cast<const u4*>(m.p + at - off), hi = *reinterpret_cast<const u4*>(m.p + at - off + 8);
+    u8 w = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    w = off & 4 ? __builtin_shufflevector(w, w, 2, 3, 4, 5, 6, 7, 7, 7) : w;
+    w = off & 2 ? __builtin_shufflevector(w, w, 1, 2, 3, 4, 5, 6, 7, 7) : w;
+    u4 o;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = c + e < n ? row[c + e] : (bf16)0.f;
+    for (int i = 0; i < 4; ++i) o[i] = __builtin_amdgcn_alignbyte(w[i + 1], w[i], 2 * (off & 1));
+    v = __builtin_bit_cast(bf16x8, o);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c + e < m.cols ? m.p[at + e] : (bf16)0.f;
+  }
+#pragma unroll
+  for (int e = 1; e < 8; ++e) v[e] = c + e < m.cols ? v[e] : (bf16)0.f;
   return v;
 }
 
@@ -73,59 +103,170 @@ __device__ __forceinline__ void to_lds(bf16* t, int row, int c, const bf16x8& v)
   for (int e = 0; e < 4; ++e) d[e] = s[e];
 }
 
-// out[c][r] = in[r][c] for r < rows, zeros for r up to rows_pad
-__global__ void __launch_bounds__(256) transpose_kernel(const bf16* in, int64_t ld, int rows, int cols, bool wide, bf16* out,
-                                                        int64_t ldo, int rows_pad) {
-  __shared__ bf16 t[kTP * kTPitch];
-  const int c0 = blockIdx.x * kTP, r0 = blockIdx.y * kTP;
+// tile (c0, r0) of out[c][r] = in[r][c] for r < rows, zeros for r up to rows_pad
+__device__ __forceinline__ void transpose_tile(bf16* t, const Source& in, int c0, int r0, bf16* out, int64_t ldo, int rows_pad) {
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int i = k * 256 + threadIdx.x;
     const int c = (i & 7) * 8, r = i >> 3;
-    bf16x8 v = {};
-    if (r0 + r < rows) v = get8(in + (int64_t)(r0 + r) * ld, c0 + c, cols, wide);
-    to_lds(t, r, c, v);
+    to_lds(t, r, c, get8(in, r0 + r, c0 + c));
   }
   __syncthreads();
-  put_transposed(t, out, ldo, r0, c0, cols, rows_pad);
+  put_transposed(t, out, ldo, r0, c0, in.cols, rows_pad);
 }
 
-// dG, dU of a 64 x 64 tile: dgu[m][f], dgu[m][Fp + f] and dgut[f][m], dgut[F + f][m]
+// what gated_prepare_kernel makes, in tiles of 64 x 64: first the gradients of
+// the projections, then the transposes
+struct Prepare {
+  Source dh, gate, up;  // [M][F]
+  bf16* dgu;            // [M][2 Fp]
+  bf16* dgut;           // [2 F][Mp]
+  int Fp, Mp, tiles_g;
+  Source in[3];         // X, and Wg, Wu or nothing
+  bf16* out[3];
+  int64_t ldo[3];
+  int rows_pad[3], tiles[3];
+};
 template <int ACT>
-__global__ void __launch_bounds__(256) gated_grad_kernel(const bf16* dh, const bf16* gate, const bf16* up, int M, int F, int Fp,
-                                                         int Mp, bool wide, bf16* dgu, bf16* dgut) {
-  __shared__ bf16 tg[kTP * kTPitch], tu[kTP * kTPitch];
-  const int f0 = blockIdx.x * kTP, m0 = blockIdx.y * kTP;
+__global__ void __launch_bounds__(256) gated_prepare_kernel(Prepare p) {
+  __shared__ __attribute__((aligned(16))) bf16 tg[kTP * kTPitch], tu[kTP * kTPitch];
+  int b = blockIdx.x;
+  if (b >= p.tiles_g) {
+    b -= p.tiles_g;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      if (b >= 0 && b < p.tiles[k]) {
+        const int nc = cdiv(p.in[k].cols, kTP);
+        transpose_tile(tg, p.in[k], b % nc * kTP, b / nc * kTP, p.out[k], p.ldo[k], p.rows_pad[k]);
+      }
+      b -= p.tiles[k];
+    }
+    return;
+  }
+  const int F = p.dh.cols, M = p.dh.rows, Fp = p.Fp, nf = cdiv(F, kTP);
+  const int f0 = b % nf * kTP, m0 = b / nf * kTP;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int i = k * 256 + threadIdx.x;
     const int c = (i & 7) * 8, r = i >> 3, m = m0 + r, f = f0 + c;
     bf16x8 vg = {}, vu = {};
     if (m < M && f < F) {
-      const int64_t at = (int64_t)m * F;
-      const bf16x8 d8 = get8(dh + at, f, F, wide), g8 = get8(gate + at, f, F, wide), u8 = get8(up + at, f, F, wide);
-      float a[8], b[8];
+      const bf16x8 d8 = get8(p.dh, m, f), g8 = get8(p.gate, m, f), u8 = get8(p.up, m, f);
+      float a[8], u[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         float fv, dv;
         gate_slope<ACT>((float)g8[e], fv, dv);
         const float d = (float)d8[e];
-        a[e] = d * (float)u8[e] * dv;
-        b[e] = d * fv;
+        a[e] = f + e < F ? d * (float)u8[e] * dv : 0.f;
+        u[e] = f + e < F ? d * fv : 0.f;
       }
       vg = cvt8(a);
-      vu = cvt8(b);
+      vu = cvt8(u);
     }
     if (m < M && f < Fp) {
-      store8(dgu + (int64_t)m * 2 * Fp + f, vg);
-      store8(dgu + (int64_t)m * 2 * Fp + Fp + f, vu);
+      store8(p.dgu + (int64_t)m * 2 * Fp + f, vg);
+      store8(p.dgu + (int64_t)m * 2 * Fp + Fp + f, vu);
     }
     to_lds(tg, r, c, vg);
     to_lds(tu, r, c, vu);
   }
   __syncthreads();
-  put_transposed(tg, dgut, Mp, m0, f0, F, Mp);
-  put_transposed(tu, dgut + (int64_t)F * Mp, Mp, m0, f0, F, Mp);
+  put_transposed(tg, p.dgut, p.Mp, m0, f0, F, p.Mp);
+  put_transposed(tu, p.dgut + (int64_t)F * p.Mp, p.Mp, m0, f0, F, p.Mp);
+}
+
+// dX of few rows, from the weights as they lie: part[s][m][d], the sum over
+// K-blocks [s per, (s + 1) per) of 128 rows of Wg, then of Wu.
+//
+// A workgroup owns 128 columns d; a block of 128 f x 128 d goes to LDS as it is
+// ([f][d], rows of 256 bytes) and is read across by ds_read_b64_tr_b16, which
+// gives a lane four f of one d: MFMA fragments with K along f.  dG and dU come
+// straight from memory, they are small and stay in cache.  One image and two
+// barriers a block: several workgroups a CU keep the memory busy in each
+// other's pauses.  Slot s of LDS row r holds piece s ^ (2 (r & 3) + 8 (r >> 3 & 1)):
+// the 8 rows that a read's 32 lanes touch fall on 8 different 32-byte ranges.
+constexpr int kDxF = 128, kDxD = 128;
+struct DxRows {
+  const bf16* w[2];
+  int64_t ldw;
+  const bf16* dgu;
+  int M, D, F, Fp, per;  // per: blocks a split
+  float* part;
+};
+template <int FB>
+__global__ void __launch_bounds__(256) gated_dx_rows_kernel(DxRows p) {
+  __shared__ __attribute__((aligned(128))) bf16 lds[kDxF * kDxD];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r16 = lane & 15, g = lane >> 4;
+  const int d0 = blockIdx.x * kDxD;
+  const int nb = cdiv(p.F, kDxF);  // blocks a matrix
+  const int b0 = blockIdx.y * p.per, b1 = min(2 * nb, b0 + p.per);
+
+  // load j of wave w: rows 16 j + 4 w + lane / 16, 16 pieces of 8 columns
+  const int lr = 4 * wave + (lane >> 4);
+  auto swz = [](int r) { return 2 * (r & 3) + 8 * ((r >> 3) & 1); };
+  f32x4 acc[2][FB];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < FB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const bf16* row[FB];  // of dG | dU
+#pragma unroll
+  for (int j = 0; j < FB; ++j) row[j] = p.dgu + (int64_t)min(16 * j + r16, p.M - 1) * 2 * p.Fp;
+
+  for (int b = b0; b < b1; ++b) {
+    const int h = b >= nb, f0 = (b - h * nb) * kDxF;
+    const bf16* w = p.w[h] + (int64_t)f0 * p.ldw;
+#pragma unroll
+    for (int j = 0; j < kDxF / 16; ++j) {
+      const int r = 16 * j + lr;
+      const int c = min(d0 + 8 * ((lane & 15) ^ swz(r)), p.D - 8);  // columns past the end: the last ones again
+      const char* s = reinterpret_cast<const char*>(w + (int64_t)r * p.ldw + c);
+      if (f0 + r >= p.F) s = reinterpret_cast<const char*>(tile::kZero16);
+      __builtin_amdgcn_global_load_lds((tile::gvoid*)s, (tile::lvoid*)(lds + (16 * j + 4 * wave) * kDxD), 16, 0, 0);
+    }
+    bf16x8 x[kDxF / 32][FB];
+#pragma unroll
+    for (int k = 0; k < kDxF / 32; ++k) {
+      const int f = f0 + 32 * k + 8 * g;
+#pragma unroll
+      for (int j = 0; j < FB; ++j) {
+        x[k][j] = load8(row[j] + h * p.Fp + min(f, p.Fp - 8));
+        if (f >= p.Fp) x[k][j] = bf16x8{};
+      }
+    }
+    __syncthreads();  // the block has landed (every wave waits for its loads before the barrier)
+#pragma unroll
+    for (int k = 0; k < kDxF / 32; ++k) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = 32 * wave + 16 * i + 4 * (r16 & 3);  // this lane's 4 columns of the rows that it reads for
+        bf16x4 q[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int r = 32 * k + 8 * g + 4 * t + (r16 >> 2);
+          q[t] = tr4(lds + r * kDxD + (((c >> 3) ^ swz(r)) << 3) + (c & 7));
+        }
+        const bf16x8 a = __builtin_shufflevector(q[0], q[1], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+        for (int j = 0; j < FB; ++j) acc[i][j] = mma(acc[i][j], a, x[k][j]);
+      }
+    }
+    __syncthreads();  // read by all
+  }
+  // lane (r16, g): columns 4 g .. of fragment i, row r16 of group j
+  float* out = p.part + (int64_t)blockIdx.y * p.M * p.D;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int d = d0 + 32 * wave + 16 * i + 4 * g;
+    if (d >= p.D) continue;  // (D is a multiple of 8)
+#pragma unroll
+    for (int j = 0; j < FB; ++j) {
+      const int m = 16 * j + r16;
+      if (m < p.M) *reinterpret_cast<f32x4*>(out + (int64_t)m * p.D + d) = acc[i][j];
+    }
+  }
 }
 
 // C[b][a] of the tile loop, bf16, or one of gridDim.y partial sums over K in fp32
@@ -183,7 +324,7 @@ __global__ void __launch_bounds__(256) sum_partials_kernel(const float* part, in
 }
 
 // outputs a workgroup, workgroups a CU, us a step (tile_gemm.h: Form)
-constexpr tile::Form kForms[] = {{64, 64, 2, 0.22f, 0.5f}, {128, 64, 2, 0.33f, 0.67f}, {128, 128, 2, 0.46f, 0.97f},
+constexpr tile::Form kForms[] = {{64, 64, 2, 0.27f, 0.5f}, {128, 64, 2, 0.33f, 0.67f}, {128, 128, 2, 0.46f, 0.97f},
                                  {256, 256, 1, 1.55f, 1.55f}};
 // How a product is done: its form, and into how many sums over K it is split
 // where it has few tiles (1024 x 777 outputs, K = 5472: 37.0 us in 56 tiles of
@@ -215,9 +356,23 @@ How how_of(int64_t arows, int64_t brows, int64_t kbytes) {
   return best;
 }
 
+// dX from the weights as they are: for few rows, whole aligned pieces
+bool dx_rows_fit(const GatedBwdParams& p) {
+  const auto a = reinterpret_cast<uintptr_t>(p.wg) | reinterpret_cast<uintptr_t>(p.wu);
+  return p.M <= 128 && p.D % 8 == 0 && p.ldw % 8 == 0 && a % 16 == 0;
+}
+// its K splits: three workgroups a CU, fewer where the partial sums' bytes
+// (8 M D a split, written and read) would pass a quarter of the weights'
+int dx_rows_splits(int M, int D, int F) {
+  const int64_t cols = cdiv(D, kDxD), blocks = 2 * (int64_t)cdiv(F, kDxF);
+  const int64_t most = std::max<int64_t>(1, F / (8 * (int64_t)M));
+  return (int)std::max<int64_t>(1, std::min({blocks, (3 * tile::kCus + cols - 1) / cols, std::max<int64_t>(most, 256 / cols)}));
+}
+
 struct Plan {
   int Fp, Mp;
   How x, w;  // dX and dW
+  int rows;  // K splits of dX by gated_dx_rows_kernel
   int64_t dgu, dgut, wt, xt, part, total;  // byte offsets
 };
 Plan plan_of(int M, int D, int F) {
@@ -236,8 +391,10 @@ Plan plan_of(int M, int D, int F) {
   q.dgut = take(2 * 2 * (int64_t)F * q.Mp);
   q.wt = take(2 * (int64_t)D * 2 * q.Fp);
   q.xt = take(2 * (int64_t)D * q.Mp);
+  q.rows = M <= 128 ? dx_rows_splits(M, D, F) : 0;
+  const int64_t pr = 4 * (int64_t)q.rows * M * D;
   const int64_t px = q.x.S > 1 ? 4 * q.x.S * (int64_t)M * D : 0, pw = q.w.S > 1 ? 4 * q.w.S * 2 * (int64_t)F * D : 0;
-  q.part = take(std::max(px, pw));
+  q.part = take(std::max({px, pw, pr}));
   q.total = at;
   return q;
 }
@@ -277,12 +434,6 @@ void product(const char* a, int arows, const char* b, int brows, int64_t kbytes,
   }
 }
 
-void transpose(const void* in, int64_t ld, int rows, int cols, bf16* out, int64_t ldo, int rows_pad, hipStream_t s) {
-  const bool wide = reinterpret_cast<uintptr_t>(in) % 16 == 0 && ld % 8 == 0 && cols % 8 == 0;
-  hipLaunchKernelGGL(transpose_kernel, dim3((unsigned)cdiv(cols, kTP), (unsigned)cdiv(rows, kTP)), dim3(256), 0, s,
-                     static_cast<const bf16*>(in), ld, rows, cols, wide, out, ldo, rows_pad);
-}
-
 }  // namespace
 
 int64_t gated_backward_bytes(int M, int D, int F) { return plan_of(M, D, F).total; }
@@ -301,19 +452,45 @@ void gated_backward(const GatedBwdParams& p, hipStream_t s) {
   bf16* xt = reinterpret_cast<bf16*>(w + q.xt);
   float* part = reinterpret_cast<float*>(w + q.part);
 
-  const bool wide = p.F % 8 == 0 && (reinterpret_cast<uintptr_t>(p.dh) | reinterpret_cast<uintptr_t>(p.gate) |
-                                     reinterpret_cast<uintptr_t>(p.up)) % 16 == 0;
-  const dim3 grid((unsigned)cdiv(p.F, kTP), (unsigned)cdiv(p.M, kTP));
+  const bool rows = dx_rows_fit(p);
+  auto tiles = [](int r, int c) { return cdiv(r, kTP) * cdiv(c, kTP); };
+  Prepare t;
+  t.dh = source(p.dh, p.F, p.M, p.F);
+  t.gate = source(p.gate, p.F, p.M, p.F);
+  t.up = source(p.up, p.F, p.M, p.F);
+  t.dgu = dgu; t.dgut = dgut;
+  t.Fp = q.Fp; t.Mp = q.Mp;
+  t.tiles_g = tiles(p.M, p.F);
+  t.in[0] = source(p.x, p.ldx, p.M, p.D);
+  t.in[1] = source(p.wg, p.ldw, p.F, p.D);
+  t.in[2] = source(p.wu, p.ldw, p.F, p.D);
+  t.out[0] = xt; t.ldo[0] = t.rows_pad[0] = q.Mp;
+  t.out[1] = wt; t.out[2] = wt + q.Fp;
+  t.ldo[1] = t.ldo[2] = 2 * q.Fp;
+  t.rows_pad[1] = t.rows_pad[2] = q.Fp;
+  t.tiles[0] = tiles(p.M, p.D);
+  t.tiles[1] = t.tiles[2] = rows ? 0 : tiles(p.F, p.D);
+  const dim3 grid((unsigned)(t.tiles_g + t.tiles[0] + t.tiles[1] + t.tiles[2]));
   with_gate(p.act, [&](auto k) {
-    hipLaunchKernelGGL((gated_grad_kernel<decltype(k)::v>), grid, dim3(256), 0, s, static_cast<const bf16*>(p.dh),
-                       static_cast<const bf16*>(p.gate), static_cast<const bf16*>(p.up), p.M, p.F, q.Fp, q.Mp, wide, dgu,
-                       dgut);
+    hipLaunchKernelGGL((gated_prepare_kernel<decltype(k)::v>), grid, dim3(256), 0, s, t);
   });
-  transpose(p.wg, p.ldw, p.F, p.D, wt, 2 * q.Fp, q.Fp, s);
-  transpose(p.wu, p.ldw, p.F, p.D, wt + q.Fp, 2 * q.Fp, q.Fp, s);
-  transpose(p.x, p.ldx, p.M, p.D, xt, q.Mp, q.Mp, s);
-  product(reinterpret_cast<const char*>(wt), p.D, reinterpret_cast<const char*>(dgu), p.M, 4 * (int64_t)q.Fp,
-          static_cast<bf16*>(p.dx), part, q.x, s);
+  if (rows) {
+    const int blocks = 2 * cdiv(p.F, kDxF);
+    DxRows d{{static_cast<const bf16*>(p.wg), static_cast<const bf16*>(p.wu)}, p.ldw, dgu, p.M, p.D, p.F, q.Fp,
+             cdiv(blocks, q.rows), part};
+    const int S = cdiv(blocks, d.per);
+    const dim3 g((unsigned)cdiv(p.D, kDxD), (unsigned)S);
+    if (p.M <= 16) hipLaunchKernelGGL(gated_dx_rows_kernel<1>, g, dim3(256), 0, s, d);
+    else if (p.M <= 32) hipLaunchKernelGGL(gated_dx_rows_kernel<2>, g, dim3(256), 0, s, d);
+    else if (p.M <= 64) hipLaunchKernelGGL(gated_dx_rows_kernel<4>, g, dim3(256), 0, s, d);
+    else hipLaunchKernelGGL(gated_dx_rows_kernel<8>, g, dim3(256), 0, s, d);
+    const int64_t n = (int64_t)p.M * p.D;
+    hipLaunchKernelGGL(sum_partials_kernel, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, s, part, n, S,
+                       static_cast<bf16*>(p.dx));
+  } else {
+    product(reinterpret_cast<const char*>(wt), p.D, reinterpret_cast<const char*>(dgu), p.M, 4 * (int64_t)q.Fp,
+            static_cast<bf16*>(p.dx), part, q.x, s);
+  }
   product(reinterpret_cast<const char*>(xt), p.D, reinterpret_cast<const char*>(dgut), 2 * p.F, 2 * (int64_t)q.Mp,
           static_cast<bf16*>(p.dw), part, q.w, s);
   MCC_CHECK(hipGetLastError() == hipSuccess, "gated_linear_bwd: launch failed");

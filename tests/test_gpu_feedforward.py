@@ -494,3 +494,256 @@ def test_distill_gradient_against_differences(cuda):
         num = (side[0] - side[1]) / (2 * h)
         # h^2 / 6 of a third derivative below 1, the differences' rounding, and fp32 in the kernel
         assert abs(dz[at].item() - num) < h * h + 1e-15 / h * 100 + 1e-6
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# strides, streams, graphs, a run of them together
+# ---------------------------------------------------------------------------------------------------------------
+def wide_view(t, left, right):
+    """t's values as columns of a wider matrix whose other columns are NaN (127 for int8)."""
+    rows, cols = t.shape
+    fill = 127 if t.dtype == torch.int8 else float("nan")
+    big = torch.full((rows, left + cols + right), fill, dtype=t.dtype, device=t.device)
+    view = big[:, left : left + cols]
+    view.copy_(t)
+    return view
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("left,right", [(0, 8), (8, 8), (3, 0), (1, 4)])
+@pytest.mark.parametrize("M,D,F", [(3, 72, 40), (20, 64, 4500), (150, 104, 200), (90, 100, 130)])
+def test_gated_linear_strided(cuda, M, D, F, left, right):
+    case = gated_bwd_case(gen(4, cuda), M, D, F)
+    dh, x, wg, wu, gate, up = case
+    v = [wide_view(t, left, right) for t in case]
+    gated_check(x, wg, wu, "silu", ops.gated_linear(v[1], v[2], v[3], "silu", save=True), True)
+    gated_bwd_check(*case, "silu", ops.gated_linear_bwd(*v, "silu"))
+    # the two weights of one pitch each, a transposed input
+    xt = x.t().contiguous().t()
+    gated_check(x, wg, wu, "silu", ops.gated_linear(xt, wg, v[3], "silu", save=True), True)
+    gated_bwd_check(*case, "silu", ops.gated_linear_bwd(dh.t().contiguous().t(), xt, v[2], wu, gate, v[5], "silu"))
+    # one row of x for all tokens
+    same = x[:1].expand(M, D)
+    gated_check(same, wg, wu, "silu", ops.gated_linear(same, wg, wu, "silu"), False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("left,right", [(0, 16), (16, 16), (3, 0)])
+@pytest.mark.parametrize("M,N,K", [(3, 40, 96), (200, 130, 96), (90, 33, 100)])
+def test_linear_i8_strided(cuda, M, N, K, left, right):
+    x, sx, w, sw, b = i8_case(gen(4, cuda), M, N, K)
+    sx2, sw2, b2 = (torch.stack([t, torch.full_like(t, float("nan"))], 1)[:, 0] for t in (sx, sw, b))
+    i8_check(x, sx, w, sw, b, "none", ops.linear_i8(wide_view(x, left, right), sx2, wide_view(w, left, right), sw2, b2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("left,right", [(0, 8), (8, 8), (3, 0)])
+@pytest.mark.parametrize("M,D", [(5, 96), (3, 4096), (2, 10007)])
+def test_rmsnorm_i8_strided(cuda, M, D, left, right, dtype):
+    g = gen(4, cuda)
+    x, r = randn(g, M, D, dtype=dtype), randn(g, M, D, dtype=dtype)
+    w = randn(g, D, dtype=dtype)
+    norm_check(x, w, r, 1e-6, ops.rmsnorm_i8(wide_view(x, left, right), torch.stack([w, w], 1)[:, 0],
+                                             wide_view(r, left, right)))
+
+
+@pytest.mark.gpu
+def test_empty_batches(cuda):
+    g = gen(1, cuda)
+    x, wg = randn(g, 0, 64), randn(g, 32, 64)
+    h, gate, up = ops.gated_linear(x, wg, wg, save=True)
+    assert h.shape == gate.shape == up.shape == (0, 32)
+    dx, dwg, dwu = ops.gated_linear_bwd(h, x, wg, wg, gate, up)
+    assert dx.shape == (0, 64) and not dwg.any() and not dwu.any() and dwg.shape == dwu.shape == (32, 64)
+    q, s, v = ops.rmsnorm_i8(x, wg[0], x)
+    assert q.shape == v.shape == (0, 64) and s.shape == (0,)
+    wq, sw = torch.ones(8, 64, dtype=torch.int8, device=cuda), torch.ones(8, device=cuda)
+    assert ops.linear_i8(q, s, wq, sw).shape == (0, 8)
+    dz, loss = ops.distill_kl(x, torch.empty(0, 3, device=cuda), torch.empty(0, 3, dtype=torch.int64, device=cuda))
+    assert dz.shape == (0, 64) and loss.shape == (0,)
+
+
+def serving(x, r, w, w1, s1, b1):
+    """A quantised projection behind its norm."""
+    q, s, v = ops.rmsnorm_i8(x, w, r)
+    return ops.linear_i8(q, s, w1, s1, b1, "relu"), v
+
+
+def training(x, wg, wu, head, tv, ti):
+    """A student's gated block and head on a teacher's top logits: every gradient, and the loss."""
+    h, gate, up = ops.gated_linear(x, wg, wu, "silu", save=True)
+    z = ops.linear(h, head)
+    dz, loss = ops.distill_kl(z, tv, ti, temperature=2.0, scale=1.0 / x.shape[0])
+    dhead, _ = ops.linear_wgrad(dz, h)
+    dh = ops.linear_dgrad(dz, head)
+    dx, dwg, dwu = ops.gated_linear_bwd(dh, x, wg, wu, gate, up, "silu")
+    return [loss, dx, dwg, dwu, dhead]
+
+
+def training_case(g, M=200, D=96, F=160, N=104, K=8):
+    z, tv, ti = distill_case(g, M, N, K)
+    return (randn(g, M, D), randn(g, F, D, std=D**-0.5), randn(g, F, D, std=D**-0.5), randn(g, N, F, std=F**-0.5), tv, ti)
+
+
+@pytest.mark.gpu
+def test_training_run_against_autograd(cuda):
+    """The chain's gradients against torch's own derivative of the same chain in 64 bits.  Nine roundings to bf16 lie on
+    the longest way (h, z, dz, dh, gate, up, dG, dU, the gradient): each moves a sum of independent terms by at most
+    2^-8 of its terms' root sum of squares, so the whole gradient by at most 9 * 2^-8 of its norm times what
+    cancellation in the steps between costs (a factor of 3 here: |p - q| is about a third of |p| + |q|)."""
+    x, wg, wu, head, tv, ti = training_case(gen(3, cuda))
+    got = training(x, wg, wu, head, tv, ti)
+    leaf = [t.to(D64).requires_grad_() for t in (x, wg, wu, head)]
+    h = torch.nn.functional.silu(leaf[0] @ leaf[1].t()) * (leaf[0] @ leaf[2].t())
+    loss = distill64(h @ leaf[3].t(), tv, ti, 2.0, 1.0)[1]
+    (loss.sum() / x.shape[0]).backward()
+    assert ((got[0] - loss.detach()).abs() <= 2.0**-5 * (loss.detach().abs() + 1)).all()
+    for a, b in zip(got[1:], leaf):
+        rel = ((a.to(D64) - b.grad).norm() / b.grad.norm()).item()
+        assert rel < 27 * 2.0**-8, rel
+
+
+@pytest.mark.gpu
+def test_serving_run(cuda):
+    g = gen(3, cuda)
+    M, D, N = 70, 256, 120
+    x, r, w = randn(g, M, D), randn(g, M, D), randn(g, D)
+    _, _, w1, s1, b1 = i8_case(g, 1, N, D)
+    y, v = serving(x, r, w, w1, s1, b1)
+    s = x.to(D64) + r.to(D64)
+    n = s / torch.sqrt((s * s).mean(1, keepdim=True) + 1e-6) * w.to(D64)
+    W = w1.to(D64) * s1.to(D64)[:, None]
+    ref = n @ W.t() + b1.to(D64)
+    # quantising moves every value by at most half a step
+    err = (n.abs().amax(1, keepdim=True) / 127 * (0.5 + 1e-3)) @ W.abs().sum(1)[None, :]
+    within(y, ref.clamp(min=0), err + EPS_BF16 * (ref.abs() + err) + 1e-6, "y")
+    assert torch.equal(v, (x.float() + r.float()).bfloat16())
+
+
+@pytest.mark.gpu
+def test_runs_repeat_exactly_on_any_stream(cuda):
+    """The same bits again, on another stream, and from two streams at once."""
+    case, big = training_case(gen(3, cuda)), training_case(gen(4, cuda), 700, 520, 1000, 3000, 16)
+    for c in (case, big):
+        one = training(*c)
+        for a, b in zip(one, training(*c)):
+            assert torch.equal(a, b)
+        s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        out = {}
+        for rep in range(3):
+            for s in (s1, s2):
+                with torch.cuda.stream(s):
+                    out[s] = training(*c)
+        torch.cuda.synchronize()
+        for s in (s1, s2):
+            for a, b in zip(one, out[s]):
+                assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_captured_runs(cuda):
+    """Training and serving runs captured into two graphs, replayed in turn with new inputs and eager work between."""
+    g = gen(5, cuda)
+    t_in = [t.clone() for t in training_case(g)]
+    s_in = [randn(g, 9, 256), randn(g, 9, 256), randn(g, 256), *i8_case(g, 1, 120, 256)[2:]]
+    rows_in = gated_bwd_case(g, 7, 136, 520)  # few rows: other kernels than t_in's
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        training(*t_in), serving(*s_in), ops.gated_linear_bwd(*rows_in)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        o1 = training(*t_in)
+    with torch.cuda.graph(g2):
+        o2 = [*serving(*s_in), *ops.gated_linear_bwd(*rows_in)]
+    for rep in range(4):
+        new = training_case(gen(10 + rep, cuda))
+        for a, b in zip(t_in, new):
+            a.copy_(b)
+        s_in[0].copy_(randn(gen(20 + rep, cuda), 9, 256))
+        rows_in[0].copy_(randn(gen(30 + rep, cuda), 7, 520))
+        g1.replay()
+        g2.replay()
+        g1.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(o1, training(*t_in)):
+            assert torch.equal(a, b), rep
+        for a, b in zip(o2, [*serving(*s_in), *ops.gated_linear_bwd(*rows_in)]):
+            assert torch.equal(a, b), rep
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# refusals (the arguments are looked at before the device: these run without a GPU)
+# ---------------------------------------------------------------------------------------------------------------
+def refused(match, f, *a, **k):
+    with pytest.raises(RuntimeError, match=match):
+        f(*a, **k)
+
+
+def test_refusals():
+    b, f = torch.bfloat16, torch.float32
+    x, w, h = torch.zeros(4, 16, dtype=b), torch.zeros(8, 16, dtype=b), torch.zeros(4, 8, dtype=b)
+    refused("unknown activation", ops.gated_linear, x, w, w, "swish")
+    refused("x has dtype", ops.gated_linear, x.float(), w, w)
+    refused("x must be a 2-D", ops.gated_linear, x[0], w, w)
+    refused("w_gate has shape", ops.gated_linear, x, w[:, :8], w)
+    refused("w_up has shape", ops.gated_linear, x, w, w[:4])
+    refused("empty weights", ops.gated_linear, x, w[:0], w[:0])
+    refused("on the GPU", ops.gated_linear, x, w, w)
+    refused("unknown activation", ops.gated_linear_bwd, h, x, w, w, h, h, 3)
+    refused("dh has shape", ops.gated_linear_bwd, h[:2], x, w, w, h, h)
+    refused("gate has dtype", ops.gated_linear_bwd, h, x, w, w, h.float(), h)
+    refused("up has shape", ops.gated_linear_bwd, h, x, w, w, h, h[:, :4])
+    refused("on the GPU", ops.gated_linear_bwd, h, x, w, w, h, h)
+    q, p = torch.zeros(4, 16, dtype=torch.int8), torch.zeros(8, 16, dtype=torch.int8)
+    s4, s8 = torch.zeros(4), torch.zeros(8)
+    refused("x has dtype", ops.linear_i8, q.to(torch.uint8), s4, p, s8)
+    refused("w has shape", ops.linear_i8, q, s4, p[:, :8], s8)
+    refused("x_scale must be a vector of 4", ops.linear_i8, q, s8, p, s8)
+    refused("w_scale has dtype", ops.linear_i8, q, s4, p, s8.double())
+    refused("b must be a vector", ops.linear_i8, q, s4, p, s8, s4)
+    refused("unknown activation", ops.linear_i8, q, s4, p, s8, None, "gelu")
+    refused("out_dtype", ops.linear_i8, q, s4, p, s8, out_dtype=torch.float16)
+    refused("131071", ops.linear_i8, torch.zeros(1, 131072, dtype=torch.int8), s4[:1],
+            torch.zeros(1, 131072, dtype=torch.int8), s4[:1])
+    refused("on the GPU", ops.linear_i8, q, s4, p, s8)
+    refused("bf16 or fp32", ops.rmsnorm_i8, x.half(), x[0].half())
+    refused("w must be a vector", ops.rmsnorm_i8, x, h[0])
+    refused("w has dtype", ops.rmsnorm_i8, x, x[0].float())
+    refused("residual has shape", ops.rmsnorm_i8, x, x[0], h)
+    refused("eps", ops.rmsnorm_i8, x, x[0], eps=-1.0)
+    refused("eps", ops.rmsnorm_i8, x, x[0], eps=float("nan"))
+    refused("rows of 1 to 32768", ops.rmsnorm_i8, torch.zeros(1, 32769), torch.zeros(32769))
+    refused("on the GPU", ops.rmsnorm_i8, x, x[0])
+    t, i = torch.zeros(4, 3), torch.zeros(4, 3, dtype=torch.int64)
+    refused("bf16 or fp32", ops.distill_kl, x.half(), t, i)
+    refused("t_index has dtype", ops.distill_kl, x, t, i.short())
+    refused("t_index has shape", ops.distill_kl, x, t, i[:, :2])
+    refused("t_logits has shape", ops.distill_kl, x, t[:2], i)
+    refused("temperature", ops.distill_kl, x, t, i, temperature=0.0)
+    refused("temperature", ops.distill_kl, x, t, i, temperature=float("inf"))
+    refused("grad_dtype", ops.distill_kl, x.float(), t, i, grad_dtype=b)
+    refused("at most 1024", ops.distill_kl, x, torch.zeros(4, 1025), torch.zeros(4, 1025, dtype=torch.int64))
+    refused("no classes", ops.distill_kl, x[:, :0], t, i)
+    refused("on the GPU", ops.distill_kl, x, t, i)
+
+
+def test_native_refusals():
+    """The launchers check by themselves: bad arguments raise before anything is launched."""
+    K = ops.feedforward._K
+    err = ops.feedforward._C.MccError
+    for call in (lambda: K.gated_forward(1, 8, 8, 9, 0, 8, 0, 0, 8, 0), lambda: K.gated_forward(1, 8, 8, 0, 0, 4, 0, 0, 8, 0),
+                 lambda: K.gated_forward(1, 8, 8, 0, 2, 8, 0, 0, 8, 0), lambda: K.gated_forward(1, 0, 8, 0, 0, 8, 0, 0, 8, 0),
+                 lambda: K.gated_backward(1, 8, 8, 0, 0, 0, 0, 0, 4, 0, 0, 8, 0, 0, 0),
+                 lambda: K.linear_i8(1, 1, 131072, 0, 0, 131072, 0, 0, 131072, 0, 0, 0, False),
+                 lambda: K.linear_i8(1, 1, 16, 3, 0, 16, 0, 0, 16, 0, 0, 0, False),
+                 lambda: K.rmsnorm_i8(1, 40000, False, 0, 40000, 0, 0, 0, 0.0, 0, 0, 0),
+                 lambda: K.distill_kl(1, 8, 2000, 0, 8, True, 0, True, 0, True, 1.0, 1.0, 0, True, 0, 0),
+                 lambda: K.distill_kl(1, 8, 1, 0, 8, True, 0, True, 0, True, 0.0, 1.0, 0, True, 0, 0),
+                 lambda: K.distill_kl(1, 200000, 1, 0, 200000, True, 0, True, 0, True, 1.0, 1.0, 0, True, 0, 0)):
+        with pytest.raises(err):
+            call()
