@@ -81,7 +81,7 @@ __device__ __forceinline__ bf16x8 get8(const Source& m, int r, int c) {
 }
 
 // the 64 x 64 tile in LDS ([row][col]) to out[c0 + col][r0 + row], 8 rows a
-// store: columns below cols, rows below rows_pad (a multiple of 8)
+// store: columns below cols, rows below rows_pad (a multiple of 64)
 __device__ __forceinline__ void put_transposed(const bf16* t, bf16* out, int64_t ldo, int r0, int c0, int cols,
                                                int rows_pad) {
 #pragma unroll
@@ -323,9 +323,12 @@ __global__ void __launch_bounds__(256) sum_partials_kernel(const float* part, in
   }
 }
 
-// outputs a workgroup, workgroups a CU, us a step (tile_gemm.h: Form)
-constexpr tile::Form kForms[] = {{64, 64, 2, 0.27f, 0.5f}, {128, 64, 2, 0.33f, 0.67f}, {128, 128, 2, 0.46f, 0.97f},
-                                 {256, 256, 1, 1.55f, 1.55f}};
+// outputs a workgroup, workgroups a CU, us a step (tile_gemm.h: Form).  640 x
+// 16384 x 4096 150 / 126 / 103 / 101 / 92 us; 1024 x 8192 x 8192 216 / 176 / 133 /
+// 113 / 157 us, the last in two sums over K 104
+constexpr tile::Form kForms[] = {{64, 64, 2, 0.27f, 0.5f}, {128, 64, 2, 0.33f, 0.69f}, {128, 128, 2, 0.5f, 1.04f},
+                                 {256, 128, 1, 0.86f, 0.86f}, {256, 256, 1, 1.55f, 1.55f}};
+constexpr int kNForms = 5;
 // How a product is done: its form, and into how many sums over K it is split
 // where it has few tiles (1024 x 777 outputs, K = 5472: 37.0 us in 56 tiles of
 // 128 x 128, 15.5 in 4 sums of them and 5 to add these up; 21.8 in 208 tiles of
@@ -337,20 +340,16 @@ How how_of(int64_t arows, int64_t brows, int64_t kbytes) {
   const int64_t steps = (kbytes + 127) / 128;
   How best{0, 1};
   float least = 1e30f;
-  for (int f = 0; f < 4; ++f) {
+  for (int f = 0; f < kNForms; ++f) {
     const int64_t n = tile::workgroups(kForms[f], arows, brows);
-    // (the largest form has no split: it is for products that fill the chip)
-    for (int S = 1; S <= (f == 3 ? 1 : 16) && steps / S >= 4; S *= 2) {
+    for (int S = 1; S <= 16 && (S == 1 || steps / S >= 4); ++S) {
+      // adding the sums up: a launch, and 8 bytes of each a value
       const float join = S == 1 ? 0.f : 4.f + (float)S * arows * brows * 8.f / 4e6f;
       const float us = tile::step_us(kForms[f], n * S) * (float)((steps + S - 1) / S) + join;
       if (us < least) {
         least = us;
         best = {f, S};
       }
-    }
-    if (steps < 4 && tile::step_us(kForms[f], n) < least) {
-      least = tile::step_us(kForms[f], n);
-      best = {f, 1};
     }
   }
   return best;
@@ -377,8 +376,10 @@ struct Plan {
 };
 Plan plan_of(int M, int D, int F) {
   Plan q;
-  q.Fp = (int)round_up(F, 8);
-  q.Mp = (int)round_up(M, 8);
+  // rows of whole 128-byte lines: with rows of 7344 bytes every step's piece of a
+  // row lies on two (640 x 17134 x 3672 140 us, of 8192 bytes in proportion 96)
+  q.Fp = (int)round_up(F, 64);
+  q.Mp = (int)round_up(M, 64);
   q.x = how_of(D, M, 4 * (int64_t)q.Fp);
   q.w = how_of(D, 2 * (int64_t)F, 2 * (int64_t)q.Mp);
   int64_t at = 0;
@@ -407,7 +408,9 @@ void launch_tiles(const Operands& o, TO* out, int steps, int S, hipStream_t s) {
 template <class TO> void launch_form(int form, const Operands& o, TO* out, int steps, int S, hipStream_t s) {
   if (form == 0) launch_tiles<1, 1, 4, 2, TO>(o, out, steps, S, s);
   else if (form == 1) launch_tiles<2, 1, 3, 2, TO>(o, out, steps, S, s);
-  else launch_tiles<2, 2, 2, 2, TO>(o, out, steps, S, s);
+  else if (form == 2) launch_tiles<2, 2, 2, 2, TO>(o, out, steps, S, s);
+  else if (form == 3) launch_tiles<4, 2, 3, 1, TO>(o, out, steps, S, s);
+  else launch_tiles<4, 4, 2, 1, TO>(o, out, steps, S, s);
 }
 
 // out [brows][arows] = B A^T
@@ -423,9 +426,7 @@ void product(const char* a, int arows, const char* b, int brows, int64_t kbytes,
   MCC_CHECK(kbytes <= (1 << 23), "gated_linear_bwd: row too long");
   const int steps = (int)((kbytes + 127) / 128);
   const int per = cdiv(steps, how.S), S = cdiv(steps, per);
-  if (how.form == 3) {
-    launch_tiles<4, 4, 2, 1, bf16>(o, out, steps, 1, s);
-  } else if (S == 1) {
+  if (S == 1) {
     launch_form<bf16>(how.form, o, out, steps, 1, s);
   } else {
     launch_form<float>(how.form, o, part, per, S, s);

@@ -205,7 +205,8 @@ GATED_BWD = [(1, 64, 16), (1, 1, 1), (2, 136, 70), (3, 9, 1), (16, 512, 100), (1
              (2634, 8, 2330), (1797, 185, 1), (2073, 16, 10), (36, 141, 2829), (2763, 4656, 1), (2178, 2144, 1),
              (33, 259, 2940), (34, 1808, 3272), (91, 10, 848), (55, 8, 1024), (33, 8, 2024), (129, 4208, 3876),
              (66, 2096, 1296), (66, 1028, 1520), (33, 1035, 2904), (2144, 1170, 1), (193, 4136, 2339), (66, 4240, 2081),
-             (2078, 70, 1416), (67, 1048, 2845)]
+             (2078, 70, 1416), (67, 1048, 2845), (1870, 904, 1), (259, 3656, 2888), (2557, 1544, 2694), (8000, 520, 300),
+             (8000, 1030, 520), (6000, 2056, 1024)]
 
 
 @pytest.mark.gpu
