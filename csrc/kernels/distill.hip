@@ -445,7 +445,7 @@ void distill_kl(const DistillParams& p, hipStream_t s) {
   MCC_CHECK(p.N < (1 << 30), "distill_kl: too many classes");
   MCC_CHECK(p.K <= kDistillMaxK, "distill_kl: too many entries per row");
   MCC_CHECK(p.ldz >= p.N, "distill_kl: row pitch");
-  MCC_CHECK(p.temperature > 0.f && p.temperature < __builtin_inff(), "distill_kl: temperature must be positive");
+  MCC_CHECK(p.temperature >= 0.99e-6f && p.temperature <= 1.01e6f, "distill_kl: temperature out of range");
   MCC_CHECK(!p.z_f32 || p.dz_f32 || !p.dz, "distill_kl: a gradient of fp32 logits is fp32");
   MCC_CHECK(p.M == 0 || !chunked(p.M, p.N, p.z_f32) || p.work, "distill_kl: workspace missing");
   if (p.M == 0) return;

@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(tile::kThreads, WPE) gated_tile_kernel(GatedPa
 
   const int wave = threadIdx.x >> 6, wa = wave >> 1, wb = wave & 1;
   const bool wide = p.F % 8 == 0;
-  typedef tile::RowStore<bf16, FA / 2> Rows;
+  typedef tile::RowStore<bf16, FA / 2, FA * FB == 16> Rows;
   const Rows rows{lds + wave * Rows::kBytes};
   static_assert(4 * Rows::kBytes <= T::kLds, "row buffers fit the images");
   __syncthreads();  // every wave has read the last image
@@ -105,12 +105,13 @@ __global__ void __launch_bounds__(64 * NW) gated_rows_kernel(GatedParams p, Oper
   });
 }
 
-// outputs a workgroup (gate and projection at once), workgroups a CU, us a step:
+// outputs a workgroup (gate and projection at once), workgroups a CU, us a step and
+// for the ends:
 // 1024^3 256 workgroups of the first form 7.8 us, of the second (128) 10.3;
 // 3000 x 512 x 4096 37.0 / 31.3 / 43.9 us; 1024 x 4096 x 4096 84 / 62 / 58 / 79;
 // 4096^3 343 / 251 / 233 / 206
-constexpr tile::Form kForms[] = {{64, 64, 2, 0.27f, 0.67f}, {64, 128, 2, 0.46f, 0.97f}, {128, 128, 1, 0.9f, 0.9f},
-                                 {128, 256, 1, 1.61f, 1.61f}};
+constexpr tile::Form kForms[] = {{64, 64, 2, 0.27f, 0.67f, 1.6f}, {64, 128, 2, 0.46f, 0.97f, 3.7f},
+                                 {128, 128, 1, 0.9f, 0.9f, 3.9f}, {128, 256, 1, 1.61f, 1.61f, 5.9f}};
 
 template <int FA, int FB, int NST, int WPE, int ACT>
 void launch_tiles(const GatedParams& p, const Operands& o, hipStream_t s) {
@@ -134,10 +135,11 @@ void gated_forward(const GatedParams& p, hipStream_t s) {
   // up to 32 rows the weights' way from memory counts, which many workgroups
   // that stream share best; above, whatever the measured step times say
   const int64_t n1 = (int64_t)cdiv(p.F, 16) * cdiv(p.M, 16), n2 = (int64_t)cdiv(p.F, 16) * cdiv(p.M, 32);
-  const int form = tile::best_form(kForms, p.F, p.M);
-  const float tiles = tile::step_us(kForms[form], tile::workgroups(kForms[form], p.F, p.M));
-  const float rows1 = tile::few_rows_us(true, 1, n1);
-  if (p.M <= 16 || (p.M <= 32 ? rows1 <= tile::few_rows_us(true, 2, n2) : rows1 < tiles)) {
+  const int64_t steps = (o.kbytes + 127) / 128;
+  const int form = tile::best_form(kForms, p.F, p.M, steps);
+  const float tiles = tile::form_us(kForms[form], tile::workgroups(kForms[form], p.F, p.M), steps);
+  const float rows1 = tile::few_rows_us(true, 1, n1) * (float)steps;
+  if (p.M <= 16 || (p.M <= 32 ? rows1 <= tile::few_rows_us(true, 2, n2) * (float)steps : rows1 < tiles)) {
     const dim3 grid((unsigned)cdiv(p.F, 16), (unsigned)cdiv(p.M, 16));
     if (o.kbytes >= 4096) hipLaunchKernelGGL((gated_rows_kernel<1, 4, 8>), grid, dim3(512), 0, s, p, o);
     else hipLaunchKernelGGL((gated_rows_kernel<1, 4, 4>), grid, dim3(256), 0, s, p, o);

@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(tile::kThreads, WPE) tile_store_kernel(Operand
   const int wave = threadIdx.x >> 6, wa = wave >> 1, wb = wave & 1;
   out += (int64_t)blockIdx.y * op.arows * op.brows;
   const bool wide = op.arows % 8 == 0;
-  typedef tile::RowStore<TO, FA> Rows;
+  typedef tile::RowStore<TO, FA, FA * FB == 16 && sizeof(TO) == 2> Rows;  // (partial sums are read again at once)
   const Rows rows{lds + wave * Rows::kBytes};
   static_assert(4 * Rows::kBytes <= T::kLds, "row buffers fit the images");
   __syncthreads();  // every wave has read the last image
@@ -326,8 +326,9 @@ __global__ void __launch_bounds__(256) sum_partials_kernel(const float* part, in
 // outputs a workgroup, workgroups a CU, us a step (tile_gemm.h: Form).  640 x
 // 16384 x 4096 150 / 126 / 103 / 101 / 92 us; 1024 x 8192 x 8192 216 / 176 / 133 /
 // 113 / 157 us, the last in two sums over K 104
-constexpr tile::Form kForms[] = {{64, 64, 2, 0.27f, 0.5f}, {128, 64, 2, 0.33f, 0.69f}, {128, 128, 2, 0.5f, 1.04f},
-                                 {256, 128, 1, 0.86f, 0.86f}, {256, 256, 1, 1.55f, 1.55f}};
+constexpr tile::Form kForms[] = {{64, 64, 2, 0.27f, 0.5f, 1.f}, {128, 64, 2, 0.33f, 0.69f, 1.5f},
+                                 {128, 128, 2, 0.55f, 1.15f, 2.f}, {256, 128, 1, 0.86f, 0.86f, 3.f},
+                                 {256, 256, 1, 1.55f, 1.55f, 5.f}};
 constexpr int kNForms = 5;
 // How a product is done: its form, and into how many sums over K it is split
 // where it has few tiles (1024 x 777 outputs, K = 5472: 37.0 us in 56 tiles of
@@ -343,9 +344,9 @@ How how_of(int64_t arows, int64_t brows, int64_t kbytes) {
   for (int f = 0; f < kNForms; ++f) {
     const int64_t n = tile::workgroups(kForms[f], arows, brows);
     for (int S = 1; S <= 16 && (S == 1 || steps / S >= 4); ++S) {
-      // adding the sums up: a launch, and 8 bytes of each a value
-      const float join = S == 1 ? 0.f : 4.f + (float)S * arows * brows * 8.f / 4e6f;
-      const float us = tile::step_us(kForms[f], n * S) * (float)((steps + S - 1) / S) + join;
+      // adding the sums up: a launch and the pauses of shorter runs, and 8 bytes a value of each
+      const float join = S == 1 ? 0.f : 7.f + (float)S * arows * brows * 8.f / 4e6f;
+      const float us = tile::form_us(kForms[f], n * S, (steps + S - 1) / S) + join;
       if (us < least) {
         least = us;
         best = {f, S};

@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(tile::kThreads, WPE) i8_tile_kernel(LinearI8Pa
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r32 = lane & 31, g = lane >> 5, wa = wave >> 1, wb = wave & 1;
   const bool wide = p.N % 8 == 0;
-  typedef tile::RowStore<TO, FA> Rows;
+  typedef tile::RowStore<TO, FA, FA * FB == 16> Rows;
   const Rows rows{lds + wave * Rows::kBytes};
   // the tile's scales and biases, one of each per thread, dealt out through LDS
   float* sw = reinterpret_cast<float*>(lds + 4 * Rows::kBytes);
@@ -110,12 +110,12 @@ void launch_tiles(const LinearI8Params& p, const Operands& o, hipStream_t s) {
     hipLaunchKernelGGL((i8_tile_kernel<FA, FB, KS, NST, WPE, ACT_NONE, TO>), grid, dim3(tile::kThreads), 0, s, p, o);
 }
 
-// outputs a workgroup, workgroups a CU, us a step: 640 x 1000 x 4096 9.8 / 11.6 /
+// outputs a workgroup, workgroups a CU, us a step and for the ends: 640 x 1000 x 4096 9.8 / 11.6 /
 // 16.1 / 37.6 us, 2048^3 16.8 / 15.2 / 13.1 / 25.3, 1024 x 4096 x 4096 29.4 / 25.7
 // / 22.6 / 40.3, 4096^3 117 / 91 / 68 / 60 (and 256 x 128 tiles, which win
 // nowhere, 23.0, 17.7, 29.5, 69)
-constexpr tile::Form kForms[] = {{64, 64, 2, 0.21f, 0.45f}, {128, 64, 2, 0.28f, 0.69f}, {128, 128, 2, 0.6f, 1.03f},
-                                 {256, 256, 1, 1.75f, 1.75f}};
+constexpr tile::Form kForms[] = {{64, 64, 2, 0.21f, 0.45f, 0.6f}, {128, 64, 2, 0.28f, 0.69f, 0.8f},
+                                 {128, 128, 2, 0.6f, 1.03f, 1.2f}, {256, 256, 1, 1.75f, 1.75f, 4.f}};
 
 template <class TO> void launch(const LinearI8Params& p, hipStream_t s) {
   Operands o;
@@ -129,10 +129,11 @@ template <class TO> void launch(const LinearI8Params& p, hipStream_t s) {
   // up to 32 rows the weights' way from memory counts, which many workgroups
   // that stream share best; above, whatever the measured step times say
   const int64_t n1 = (int64_t)cdiv(p.N, 16) * cdiv(p.M, 16), n2 = (int64_t)cdiv(p.N, 16) * cdiv(p.M, 32);
-  const int form = tile::best_form(kForms, p.N, p.M);
-  const float tiles = tile::step_us(kForms[form], tile::workgroups(kForms[form], p.N, p.M));
-  const float rows1 = tile::few_rows_us(false, 1, n1);
-  if (p.M <= 16 || (p.M <= 32 ? rows1 <= tile::few_rows_us(false, 2, n2) : rows1 < tiles)) {
+  const int64_t steps = (o.kbytes + 127) / 128;
+  const int form = tile::best_form(kForms, p.N, p.M, steps);
+  const float tiles = tile::form_us(kForms[form], tile::workgroups(kForms[form], p.N, p.M), steps);
+  const float rows1 = tile::few_rows_us(false, 1, n1) * (float)steps;
+  if (p.M <= 16 || (p.M <= 32 ? rows1 <= tile::few_rows_us(false, 2, n2) * (float)steps : rows1 < tiles)) {
     const dim3 grid((unsigned)cdiv(p.N, 16), (unsigned)cdiv(p.M, 16));
     if (o.kbytes >= 4096) hipLaunchKernelGGL((i8_rows_kernel<1, 4, 8, TO>), grid, dim3(512), 0, s, p, o);
     else hipLaunchKernelGGL((i8_rows_kernel<1, 4, 4, TO>), grid, dim3(256), 0, s, p, o);

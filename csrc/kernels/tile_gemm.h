@@ -307,7 +307,12 @@ struct Tile {
 // store instruction writes whole runs of a row: straight from the lanes it would
 // write 32 rows in 16-byte pieces, and those quarter-line writes cost the int8
 // product 20 % of its time at 8192 x 12288 x 4096.
-template <class TO, int NF>
+//
+// NT: stores that do not stay in the caches.  An output of a chip-filling
+// product is larger than they are and would push out the operands that the
+// other tiles still read: int8 8192 x 12288 x 4096 with inputs that change from
+// call to call 349 -> 328 us (fp32 output 372 -> 348).
+template <class TO, int NF, bool NT = false>
 struct RowStore {
   static constexpr int kVec = 16 / (int)sizeof(TO);       // elements per 16-byte slot
   static constexpr int kSlots = 32 * NF / kVec;           // slots per row: 4, 8, 16 or 32
@@ -342,7 +347,11 @@ struct RowStore {
       for (int t = 0; t < 32 / kRows; ++t) {
         const int row = t * kRows + lane / kSlots, m = m0 + row;
         const f32x4 v = *reinterpret_cast<const f32x4*>(lds + at(row, slot));
-        if (m < M && n < N) *reinterpret_cast<f32x4*>(out + (int64_t)m * N + n) = v;
+        f32x4* q = reinterpret_cast<f32x4*>(out + (int64_t)m * N + n);
+        if (m < M && n < N) {
+          if constexpr (NT) __builtin_nontemporal_store(v, q);
+          else *q = v;
+        }
       }
     } else {
       // Rows that start anywhere: the 16-byte pieces of memory that lie wholly in
@@ -389,26 +398,29 @@ struct RowStore {
 
 // ---- choice of a tile (host) ----
 // A form of a product: workgroups of `rows_a` x `rows_b` outputs, `per_cu` of
-// them to a CU, and what a step of 128 bytes of K takes, measured in us: `one`
-// while a CU holds one workgroup, `full` while it holds all `per_cu`.
+// them to a CU, and, measured in us, what a step of 128 bytes of K takes, `one`
+// while a CU holds one workgroup, `full` while it holds all `per_cu`, and what
+// a workgroup's start and end take.
 struct Form {
   int rows_a, rows_b, per_cu;
-  float one, full;
+  float one, full, ends;
 };
 constexpr int kCus = 256;
 inline int64_t workgroups(const Form& f, int64_t arows, int64_t brows) {
   return (arows + f.rows_a - 1) / f.rows_a * ((brows + f.rows_b - 1) / f.rows_b);
 }
-// us per step of n workgroups: whole rounds of the chip, then what is left
-inline float step_us(const Form& f, int64_t n) {
+// n workgroups of `steps` steps: whole rounds of the chip, then what is left
+inline float form_us(const Form& f, int64_t n, int64_t steps) {
   const int64_t slots = (int64_t)kCus * f.per_cu, rest = n % slots;
-  return n / slots * f.full + (rest == 0 ? 0.f : rest <= kCus ? f.one : f.full);
+  const float us = n / slots * f.full + (rest == 0 ? 0.f : rest <= kCus ? f.one : f.full);
+  return us * (float)steps + f.ends * (float)((n + slots - 1) / slots);
 }
 // the form that takes least
-template <int N> inline int best_form(const Form (&f)[N], int64_t arows, int64_t brows) {
+template <int N> inline int best_form(const Form (&f)[N], int64_t arows, int64_t brows, int64_t steps) {
   int best = 0;
   for (int i = 1; i < N; ++i)
-    if (step_us(f[i], workgroups(f[i], arows, brows)) < step_us(f[best], workgroups(f[best], arows, brows))) best = i;
+    if (form_us(f[i], workgroups(f[i], arows, brows), steps) < form_us(f[best], workgroups(f[best], arows, brows), steps))
+      best = i;
   return best;
 }
 

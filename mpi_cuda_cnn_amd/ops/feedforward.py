@@ -19,7 +19,8 @@ from .. import _C
 
 _K = _C.kernels
 # the current stream's handle without the Stream object that torch.cuda.current_stream() builds (1.8 us of a call's 10)
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 _GATE = {"none": _K.GATE_NONE, "relu": _K.GATE_RELU, "tanh": _K.GATE_TANH, "silu": _K.GATE_SILU,
          "gelu": _K.GATE_GELU}
 _ACT = {"none": _K.ACT_NONE, "relu": _K.ACT_RELU, "tanh": _K.ACT_TANH}
@@ -233,6 +234,7 @@ def distill_kl(logits: torch.Tensor, t_logits: torch.Tensor, t_index: torch.Tens
     logits [M, N] (the student's, bf16 or fp32); row m of t_logits [M, K] (bf16 or fp32) holds the teacher's logits of
     the classes t_index [M, K] (int32 or int64), K <= 1024, in any order.  An entry whose class is not in [0, N) (say
     -1) or whose logit is -inf is not there; classes that occur twice add up.  With T = temperature,
+    (1e-6 to 1e6)
     q = softmax(t_logits[m] / T) over the entries that are there and p = softmax(logits[m] / T):
 
         loss[m]    = T**2 * sum_k q_k (log q_k - log p[t_index[m, k]])            fp32 [M]
@@ -249,8 +251,8 @@ def distill_kl(logits: torch.Tensor, t_logits: torch.Tensor, t_index: torch.Tens
     _matrix(t_index, "t_index", (torch.int32, torch.int64), M, K)
     if K > _K.DISTILL_MAX_K:
         _fail(f"distill_kl: at most {_K.DISTILL_MAX_K} entries per row, got {K}")
-    if not (0.0 < temperature < float("inf")):
-        _fail(f"distill_kl: temperature = {temperature} must be positive and finite")
+    if not (1e-6 <= temperature <= 1e6):
+        _fail(f"distill_kl: temperature = {temperature} must lie between 1e-6 and 1e6")
     out = logits.dtype if grad_dtype is None else grad_dtype
     if out not in (torch.float32, logits.dtype):
         _fail(f"distill_kl: unsupported grad_dtype {out} (fp32 or the logits' type)")

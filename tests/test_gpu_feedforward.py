@@ -83,7 +83,8 @@ GATED = [(1, 64, 16), (1, 8, 1), (1, 1, 3), (2, 136, 70), (16, 512, 100), (17, 2
          (64, 4104, 48), (65, 64, 64), (66, 1, 5), (100, 333, 129), (128, 128, 64), (129, 192, 65), (300, 200, 515),
          (1000, 520, 130), (4097, 64, 1030), (2050, 136, 4232),
          # the forms that the sizes above do not reach: two groups of 16 rows, 128 x 128 and 128 x 256 tiles
-         (24, 72, 4500), (31, 1032, 4099), (1030, 72, 2063), (1024, 200, 2048), (4090, 72, 4090), (4096, 136, 4096)]
+         (24, 72, 4500), (31, 1032, 4099), (1030, 72, 2063), (1024, 200, 2048), (4090, 72, 4090), (4096, 136, 4096),
+         (923, 131, 3336), (909, 67, 3297), (1371, 8, 4804), (62, 2918, 3)]
 
 
 @pytest.mark.gpu
@@ -136,7 +137,8 @@ def i8_check(x, sx, w, sw, b, act, y):
 
 I8 = [(1, 16, 16), (1, 1, 1), (3, 5, 7), (16, 100, 4096), (17, 33, 1000), (33, 64, 144), (64, 1000, 272), (65, 64, 128),
       (128, 128, 640), (130, 70, 130), (640, 1000, 512), (1030, 4100, 176), (4100, 4360, 144), (70, 17, 20000),
-      (20, 6000, 500), (32, 4097, 4112), (1500, 1999, 400), (4090, 4090, 272), (4096, 4096, 100)]
+      (20, 6000, 500), (32, 4097, 4112), (1500, 1999, 400), (4090, 4090, 272), (4096, 4096, 100), (1870, 1110, 8), (3188, 1322, 8),
+      (3468, 3641, 647)]
 
 
 @pytest.mark.gpu
@@ -206,7 +208,8 @@ GATED_BWD = [(1, 64, 16), (1, 1, 1), (2, 136, 70), (3, 9, 1), (16, 512, 100), (1
              (33, 259, 2940), (34, 1808, 3272), (91, 10, 848), (55, 8, 1024), (33, 8, 2024), (129, 4208, 3876),
              (66, 2096, 1296), (66, 1028, 1520), (33, 1035, 2904), (2144, 1170, 1), (193, 4136, 2339), (66, 4240, 2081),
              (2078, 70, 1416), (67, 1048, 2845), (1870, 904, 1), (259, 3656, 2888), (2557, 1544, 2694), (8000, 520, 300),
-             (8000, 1030, 520), (6000, 2056, 1024)]
+             (8000, 1030, 520), (6000, 2056, 1024), (5550, 4728, 193), (5861, 522, 3385), (4130, 68, 2832),
+             (5778, 136, 3466), (5704, 648, 3034)]
 
 
 @pytest.mark.gpu
