@@ -177,16 +177,16 @@ __global__ void __launch_bounds__(256) gated_prepare_kernel(Prepare p) {
 }
 
 // dX of few rows, from the weights as they lie: part[s][m][d], the sum over
-// K-blocks [s per, (s + 1) per) of 128 rows of Wg, then of Wu.
+// K-blocks [s per, (s + 1) per) of 64 rows of Wg, then of Wu.
 //
-// A workgroup owns 128 columns d; a block of 128 f x 128 d goes to LDS as it is
+// A workgroup owns 128 columns d; a block of 64 f x 128 d goes to LDS as it is
 // ([f][d], rows of 256 bytes) and is read across by ds_read_b64_tr_b16, which
 // gives a lane four f of one d: MFMA fragments with K along f.  dG and dU come
 // straight from memory, they are small and stay in cache.  One image and two
 // barriers a block: several workgroups a CU keep the memory busy in each
 // other's pauses.  Slot s of LDS row r holds piece s ^ (2 (r & 3) + 8 (r >> 3 & 1)):
 // the 8 rows that a read's 32 lanes touch fall on 8 different 32-byte ranges.
-constexpr int kDxF = 128, kDxD = 128;
+constexpr int kDxF = 64, kDxD = 128;
 struct DxRows {
   const bf16* w[2];
   int64_t ldw;
@@ -302,13 +302,24 @@ __global__ void __launch_bounds__(tile::kThreads, WPE) tile_store_kernel(Operand
   }
 }
 
-// out = the sum of S partial arrays of n, in order
+// out = the sum of S partial arrays of n, in order; eight of them in flight (one
+// after the other, 32 of 9 x 640 took 10 us)
 __global__ void __launch_bounds__(256) sum_partials_kernel(const float* part, int64_t n, int S, bf16* out) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= n) return;
   if (n % 4 == 0) {
-    f32x4 a = *reinterpret_cast<const f32x4*>(part + i);
-    for (int s = 1; s < S; ++s) {
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    int s = 0;
+    for (; s + 8 <= S; s += 8) {
+      f32x4 b[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) b[k] = *reinterpret_cast<const f32x4*>(part + (s + k) * n + i);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] += b[k][e];
+    }
+    for (; s < S; ++s) {
       const f32x4 b = *reinterpret_cast<const f32x4*>(part + s * n + i);
 #pragma unroll
       for (int e = 0; e < 4; ++e) a[e] += b[e];
@@ -316,8 +327,8 @@ __global__ void __launch_bounds__(256) sum_partials_kernel(const float* part, in
     *reinterpret_cast<bf16x4*>(out + i) = cvt4(a[0], a[1], a[2], a[3]);
   } else {
     for (int64_t e = i; e < std::min<int64_t>(i + 4, n); ++e) {
-      float a = part[e];
-      for (int s = 1; s < S; ++s) a += part[s * n + e];
+      float a = 0.f;
+      for (int s = 0; s < S; ++s) a += part[s * n + e];
       out[e] = (bf16)a;
     }
   }
@@ -325,10 +336,11 @@ __global__ void __launch_bounds__(256) sum_partials_kernel(const float* part, in
 
 // outputs a workgroup, workgroups a CU, us a step (tile_gemm.h: Form).  640 x
 // 16384 x 4096 150 / 126 / 103 / 101 / 92 us; 1024 x 8192 x 8192 216 / 176 / 133 /
-// 113 / 157 us, the last in two sums over K 104
-constexpr tile::Form kForms[] = {{64, 64, 2, 0.27f, 0.5f, 1.f}, {128, 64, 2, 0.33f, 0.69f, 1.5f},
-                                 {128, 128, 2, 0.55f, 1.15f, 2.f}, {256, 128, 1, 0.86f, 0.86f, 3.f},
-                                 {256, 256, 1, 1.55f, 1.55f, 5.f}};
+// 113 / 157 us, the last in two sums over K 104; 4096 x 8192 x 64, all ends, 31 / 21
+// / 19 / 25 / 21
+constexpr tile::Form kForms[] = {{64, 64, 2, 0.27f, 0.5f, 1.2f}, {128, 64, 2, 0.33f, 0.69f, 1.6f},
+                                 {128, 128, 2, 0.55f, 1.15f, 2.9f}, {256, 128, 1, 0.86f, 0.86f, 4.8f},
+                                 {256, 256, 1, 1.55f, 1.55f, 7.7f}};
 constexpr int kNForms = 5;
 // How a product is done: its form, and into how many sums over K it is split
 // where it has few tiles (1024 x 777 outputs, K = 5472: 37.0 us in 56 tiles of
@@ -361,12 +373,10 @@ bool dx_rows_fit(const GatedBwdParams& p) {
   const auto a = reinterpret_cast<uintptr_t>(p.wg) | reinterpret_cast<uintptr_t>(p.wu);
   return p.M <= 128 && p.D % 8 == 0 && p.ldw % 8 == 0 && a % 16 == 0;
 }
-// its K splits: three workgroups a CU, fewer where the partial sums' bytes
-// (8 M D a split, written and read) would pass a quarter of the weights'
-int dx_rows_splits(int M, int D, int F) {
-  const int64_t cols = cdiv(D, kDxD), blocks = 2 * (int64_t)cdiv(F, kDxF);
-  const int64_t most = std::max<int64_t>(1, F / (8 * (int64_t)M));
-  return (int)std::max<int64_t>(1, std::min({blocks, (3 * tile::kCus + cols - 1) / cols, std::max<int64_t>(most, 256 / cols)}));
+// its K splits: two workgroups a CU, at least two blocks each (60 rows, weights of
+// 2 x 4096 x 4096: in 8 splits 32 us, 16 22, 32 26; of 2 x 4096 x 1024: 30, 17, 11)
+int dx_rows_splits(int D, int F) {
+  return std::max(1, std::min(cdiv(F, kDxF), cdiv(2 * tile::kCus, cdiv(D, kDxD))));
 }
 
 struct Plan {
@@ -393,7 +403,7 @@ Plan plan_of(int M, int D, int F) {
   q.dgut = take(2 * 2 * (int64_t)F * q.Mp);
   q.wt = take(2 * (int64_t)D * 2 * q.Fp);
   q.xt = take(2 * (int64_t)D * q.Mp);
-  q.rows = M <= 128 ? dx_rows_splits(M, D, F) : 0;
+  q.rows = M <= 128 ? dx_rows_splits(D, F) : 0;
   const int64_t pr = 4 * (int64_t)q.rows * M * D;
   const int64_t px = q.x.S > 1 ? 4 * q.x.S * (int64_t)M * D : 0, pw = q.w.S > 1 ? 4 * q.w.S * 2 * (int64_t)F * D : 0;
   q.part = take(std::max({px, pw, pr}));
