@@ -40,7 +40,7 @@ ENG_OBJ   := $(patsubst csrc/engine/%.cpp,$(OBJ)/engine/%.o,$(ENG_SRC))
 FF_HDRS   := csrc/kernels/feedforward.h csrc/kernels/tile_gemm.h csrc/kernels/few_rows.h csrc/kernels/gate_act.h
 HDRS      := $(filter-out $(FF_HDRS),$(wildcard csrc/include/mcc/*.h csrc/kernels/*.h csrc/apps/*.h)) \
              csrc/core/cpu_kernels.inc
-FF_OBJ    := $(patsubst %,$(OBJ)/kernels/%.o,gated gated_bwd linear_i8 rmsnorm_i8 distill) $(OBJ)/bindings/module.o
+FF_OBJ    := $(patsubst %,$(OBJ)/kernels/%.o,gated gated_bwd linear_i8 rmsnorm_i8 distill pad_rows) $(OBJ)/bindings/module.o
 
 MODULE    := mpi_cuda_cnn_amd/_C$(EXT)
 BINS      := build/bin/cnn build/bin/cnn_hip build/bin/cnn_dist build/bin/test_watchdog build/bin/test_comm

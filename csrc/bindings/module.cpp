@@ -2,6 +2,7 @@
 // as raw device pointers + HIP stream handles (torch's data_ptr() and
 // current_stream().cuda_stream), so this translation unit needs no torch
 // headers and the same engine serves the native drivers and Python.
+#include <array>
 #include <cstring>
 #include <limits>
 #include <pybind11/numpy.h>
@@ -680,6 +681,20 @@ PYBIND11_MODULE(_C, m) {
         py::arg("M"), py::arg("N"), py::arg("K"), py::arg("act"), py::arg("x"), py::arg("ldx"), py::arg("sx"),
         py::arg("w"), py::arg("ldw"), py::arg("sw"), py::arg("bias"), py::arg("y"), py::arg("f32"),
         py::arg("stream") = 0);
+  // matrices: (src, dst, ld, ldd, rows, cols), pitches and columns in bytes
+  k.def("pad_rows",
+        [](const std::vector<std::array<int64_t, 6>>& ms, uintptr_t s) {
+          gpu::PadRows p;
+          MCC_CHECK(ms.size() <= 3, "pad_rows: up to three matrices");
+          for (size_t i = 0; i < ms.size(); ++i) {
+            auto& m = p.m[i];
+            m.src = ptr<void>((uintptr_t)ms[i][0]); m.dst = ptr<void>((uintptr_t)ms[i][1]);
+            m.ld = ms[i][2]; m.ldd = ms[i][3]; m.rows = ms[i][4]; m.cols = ms[i][5];
+            m.pieces = m.rows * (m.ldd / 16);
+          }
+          gpu::pad_rows(p, stream_of(s));
+        },
+        py::arg("matrices"), py::arg("stream") = 0);
   k.def("gated_backward_bytes", &gpu::gated_backward_bytes, py::arg("M"), py::arg("D"), py::arg("F"));
   k.def("gated_backward",
         [](int M, int D, int F, int act, uintptr_t dh, uintptr_t gate, uintptr_t up, uintptr_t x, int64_t ldx, uintptr_t wg,

@@ -129,5 +129,18 @@ constexpr int kDistillMaxK = 1024;
 int64_t distill_bytes(int M, int N, bool z_f32);
 void distill_kl(const DistillParams& p, hipStream_t s);
 
+// Up to three matrices copied into rows of ldd bytes (a multiple of 16), zeros
+// behind the cols bytes that exist; sources of any pitch and alignment.
+struct PadRows {
+  struct Matrix {
+    const void* src = nullptr;
+    void* dst = nullptr;
+    int64_t ld = 0, ldd = 0, rows = 0, cols = 0;
+    int64_t pieces = 0;  // rows * ldd / 16; 0: no matrix
+  };
+  Matrix m[3];
+};
+void pad_rows(const PadRows& p, hipStream_t s);
+
 }  // namespace gpu
 }  // namespace mcc

@@ -6,9 +6,9 @@ they may run on any stream, on any device and inside a captured graph) and
 have no CPU fallback.  They compute no autograd graph: a backward pass is a
 function of its own.
 
-Rows may be strided views (unit stride along the last axis).  The kernels read
-rows in 16-byte pieces: a tensor whose rows are not whole pieces, or not
-aligned to them, is copied into padded rows first (one copy per call).
+Rows may be strided views.  The kernels read rows in 16-byte pieces: tensors
+whose rows are not whole pieces, or not aligned to them, are copied into padded
+rows first, in one launch a call.
 """
 
 from __future__ import annotations
@@ -60,21 +60,31 @@ def _device(first, *more):
     return dev
 
 
-def _pieces(t, n):
-    """(t or a copy, row pitch): rows of whole, aligned 16-byte pieces of n elements, zeros behind the last column."""
-    rows, cols = t.shape
-    if cols % n == 0:
+def _pieces(dev, n, *ts):
+    """((t or a copy, row pitch), ..): rows of whole, aligned 16-byte pieces of n elements, zeros behind the last
+    column.  All copies that a call needs are made by one kernel."""
+    out, todo = [], None
+    for t in ts:
+        rows, cols = t.shape
         ld, unit = t.stride()
         if rows <= 1:
             ld = cols
-        if unit != 1 or ld < cols or ld % n or t.data_ptr() % 16:
-            t = t.clone(memory_format=torch.contiguous_format)
+        if cols % n == 0 and unit == 1 and ld >= cols and ld % n == 0 and t.data_ptr() % 16 == 0:
+            out.append((t, ld))
+            continue
+        if unit != 1 and cols > 1:
+            t = t.contiguous()
             ld = cols
-        return t, ld
-    ld = (cols + n - 1) // n * n
-    out = torch.zeros(rows, ld, dtype=t.dtype, device=t.device)
-    out[:, :cols] = t
-    return out, ld
+        pitch = (cols + n - 1) // n * n
+        copy = torch.empty(rows, pitch, dtype=t.dtype, device=dev)
+        size = t.element_size()
+        if todo is None:
+            todo = []
+        todo.append((t.data_ptr(), copy.data_ptr(), ld * size, pitch * size, rows, cols * size))
+        out.append((copy, pitch))
+    if todo is not None:
+        _run(dev, _K.pad_rows, todo)
+    return out
 
 
 def _run(dev, fn, *args):
@@ -111,9 +121,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act:
     h = torch.empty(M, F, dtype=torch.bfloat16, device=dev)
     gate, up = (torch.empty_like(h), torch.empty_like(h)) if save else (None, None)
     if M:
-        xa, ldx = _pieces(x, 8)
-        wg, ldw = _pieces(w_gate, 8)
-        wu, ldu = _pieces(w_up, 8)
+        (xa, ldx), (wg, ldw), (wu, ldu) = _pieces(dev, 8, x, w_gate, w_up)
         if ldu != ldw:  # both weights are read with one pitch
             wg, wu, ldw = wg.contiguous(), wu.contiguous(), wg.shape[1]
         _run(dev, _K.gated_forward, M, D, F, kind, xa.data_ptr(), ldx, wg.data_ptr(), wu.data_ptr(), ldw, h.data_ptr(),
@@ -145,8 +153,7 @@ def linear_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     dev = _device(x, x_scale, w, w_scale, b)
     y = torch.empty(M, N, dtype=out_dtype, device=dev)
     if M:
-        xa, ldx = _pieces(x, 16)
-        wa, ldw = _pieces(w, 16)
+        (xa, ldx), (wa, ldw) = _pieces(dev, 16, x, w)
         sx, sw = x_scale.contiguous(), w_scale.contiguous()
         bias = b.contiguous() if b is not None else None
         _run(dev, _K.linear_i8, M, N, K, _ACT[act], xa.data_ptr(), ldx, sx.data_ptr(), wa.data_ptr(), ldw, sw.data_ptr(),
@@ -233,9 +240,8 @@ def distill_kl(logits: torch.Tensor, t_logits: torch.Tensor, t_index: torch.Tens
 
     logits [M, N] (the student's, bf16 or fp32); row m of t_logits [M, K] (bf16 or fp32) holds the teacher's logits of
     the classes t_index [M, K] (int32 or int64), K <= 1024, in any order.  An entry whose class is not in [0, N) (say
-    -1) or whose logit is -inf is not there; classes that occur twice add up.  With T = temperature,
-    (1e-6 to 1e6)
-    q = softmax(t_logits[m] / T) over the entries that are there and p = softmax(logits[m] / T):
+    -1) or whose logit is -inf is not there; classes that occur twice add up.  With T = temperature
+    (1e-6 to 1e6), q = softmax(t_logits[m] / T) over the entries that are there and p = softmax(logits[m] / T):
 
         loss[m]    = T**2 * sum_k q_k (log q_k - log p[t_index[m, k]])            fp32 [M]
         dlogits[m] = scale * T * (p - q scattered to its classes)                 [M, N]

@@ -542,6 +542,21 @@ def test_linear_i8_strided(cuda, M, N, K, left, right):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("left", range(0, 17, 2))
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 5, 7), (3, 2, 17), (40, 7, 31), (5, 300, 455)])
+def test_linear_i8_rows_of_any_alignment(cuda, M, N, K, left):
+    x, sx, w, sw, b = i8_case(gen(6, cuda), M, N, K)
+    want = ops.linear_i8(x, sx, w, sw, b)
+    i8_check(x, sx, w, sw, b, "none", want)
+    got = ops.linear_i8(wide_view(x, left, left % 3), sx, wide_view(w, left + 1, left % 5), sw, b)
+    assert torch.equal(got, want)
+    # columns of a transposed matrix, and one row for all
+    assert torch.equal(ops.linear_i8(x.t().contiguous().t(), sx, w, sw, b), want)
+    same = w[:1].expand(N, K)
+    i8_check(x, sx, same, sw, b, "none", ops.linear_i8(x, sx, same, sw, b))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("left,right", [(0, 8), (8, 8), (3, 0)])
 @pytest.mark.parametrize("M,D", [(5, 96), (3, 4096), (2, 10007)])
@@ -746,6 +761,8 @@ def test_native_refusals():
                  lambda: K.gated_backward(1, 8, 8, 0, 0, 0, 0, 0, 4, 0, 0, 8, 0, 0, 0),
                  lambda: K.linear_i8(1, 1, 131072, 0, 0, 131072, 0, 0, 131072, 0, 0, 0, False),
                  lambda: K.linear_i8(1, 1, 16, 3, 0, 16, 0, 0, 16, 0, 0, 0, False),
+                 lambda: K.pad_rows([(0, 0, 8, 24, 1, 8)]), lambda: K.pad_rows([(0, 0, 8, 16, 1, 17)]),
+                 lambda: K.pad_rows([(0, 8, 8, 16, 1, 8)]), lambda: K.pad_rows([(0, 0, 8, 16, 1, 0)]),
                  lambda: K.rmsnorm_i8(1, 40000, False, 0, 40000, 0, 0, 0, 0.0, 0, 0, 0),
                  lambda: K.distill_kl(1, 8, 2000, 0, 8, True, 0, True, 0, True, 1.0, 1.0, 0, True, 0, 0),
                  lambda: K.distill_kl(1, 8, 1, 0, 8, True, 0, True, 0, True, 0.0, 1.0, 0, True, 0, 0),
