@@ -177,89 +177,142 @@ __global__ void __launch_bounds__(256) gated_prepare_kernel(Prepare p) {
 }
 
 // dX of few rows, from the weights as they lie: part[s][m][d], the sum over
-// K-blocks [s per, (s + 1) per) of 64 rows of Wg, then of Wu.
+// K-blocks s, s + S, .. of 64 rows of Wg, then of Wu.
 //
 // A workgroup owns 128 columns d; a block of 64 f x 128 d goes to LDS as it is
 // ([f][d], rows of 256 bytes) and is read across by ds_read_b64_tr_b16, which
-// gives a lane four f of one d: MFMA fragments with K along f.  dG and dU come
-// straight from memory, they are small and stay in cache.  One image and two
-// barriers a block: several workgroups a CU keep the memory busy in each
-// other's pauses.  Slot s of LDS row r holds piece s ^ (2 (r & 3) + 8 (r >> 3 & 1)):
-// the 8 rows that a read's 32 lanes touch fall on 8 different 32-byte ranges.
+// gives a lane four f of one d: MFMA fragments with K along f.  The
+// rows of dG or dU beside it go to LDS once for the four waves.  Three images, one
+// barrier a block: blocks b + 1 and b + 2 are on their way while b is multiplied.
+// Slot s of LDS row r holds piece s ^ (2 (r & 3) + 8 (r >> 3 & 1)): the 8 rows that
+// a read's 32 lanes touch fall on 8 different 32-byte ranges.
+//
+// Bound by the weights' bytes: 2 x 12288 x 4096 (201 MB) take 51 us with 1 row, 60
+// with 128, 3.9 and 3.4 TB/s; a read of whole rows reaches 5.7.  Blocks of 256
+// columns made it 49 and 62 (2 x 4096 x 1024: 14.4 us for 11.5), 2, 3 or 4 images
+// and 1 to 4 workgroups a CU the same within 10 %.  With dG and dU from the caches
+// into each wave's registers 128 rows took 135 us: 64 KB a block from the caches
+// beside 16 KB of weights.
 constexpr int kDxF = 64, kDxD = 128;
+constexpr int kDxI = kDxD / 64;            // fragments of 16 columns a wave
+constexpr int kDxRows = 2048 / kDxD;       // rows of weights that one load of the four waves covers
+constexpr int kDxLoads = kDxF / kDxRows;
 struct DxRows {
   const bf16* w[2];
   int64_t ldw;
   const bf16* dgu;
-  int M, D, F, Fp, per;  // per: blocks a split
+  int M, D, F, Fp;
   float* part;
 };
+// Two fragments of the weights, and the wait for them in the same block: before
+// the builtin of such a read the compiler waits for the next block's loads too.
+template <int OFF> __device__ __forceinline__ void weights(bf16x8 (&a)[2], const bf16* p0, const bf16* p1) {
+  typedef short s4 __attribute__((ext_vector_type(4)));
+  s4 q[4];
+  const uint32_t l0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) bf16*)p0;
+  const uint32_t l1 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) bf16*)p1;
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %4 offset:%6\n"
+      "ds_read_b64_tr_b16 %1, %4 offset:%7\n"
+      "ds_read_b64_tr_b16 %2, %5 offset:%6\n"
+      "ds_read_b64_tr_b16 %3, %5 offset:%7\n"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(q[0]), "=&v"(q[1]), "=&v"(q[2]), "=&v"(q[3])
+      : "v"(l0), "v"(l1), "n"(OFF), "n"(OFF + 2 * 4 * kDxD)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    a[i] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(q[2 * i], q[2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+}
+// 16 bytes a lane to LDS, from base (the wave's) + at (the lane's); a buffer load
+// for the reason that Tile::run gives
+__device__ __forceinline__ void to_image(const bf16* base, uint32_t at, bf16* lds) {
+  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16*>(base), 0, -1, 0x27000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (tile::lvoid*)lds, 16, at, 0, 0, 0);
+}
 template <int FB>
 __global__ void __launch_bounds__(256) gated_dx_rows_kernel(DxRows p) {
-  __shared__ __attribute__((aligned(128))) bf16 lds[kDxF * kDxD];
+  constexpr int kW = kDxF * kDxD, kX = 16 * FB * kDxF;  // elements of an image's two parts
+  constexpr int kXLoads = FB / 2 + FB % 2;              // 32 rows a load of four waves
+  constexpr int kAhead = 2;               // blocks on their way behind the one that is multiplied
+  __shared__ __attribute__((aligned(128))) bf16 lds[(kAhead + 1) * (kW + kX)];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r16 = lane & 15, g = lane >> 4;
   const int d0 = blockIdx.x * kDxD;
   const int nb = cdiv(p.F, kDxF);  // blocks a matrix
-  const int b0 = blockIdx.y * p.per, b1 = min(2 * nb, b0 + p.per);
+  const int S = gridDim.y, n = (2 * nb - (int)blockIdx.y + S - 1) / S;  // this split's blocks
 
-  // load j of wave w: rows 16 j + 4 w + lane / 16, 16 pieces of 8 columns
-  const int lr = 4 * wave + (lane >> 4);
+  // load j of wave w: of the weights rows 16 j + 4 w + lane / 16, 16 pieces of 8
+  // columns (past the end the last ones again); of dG | dU rows 32 j + 8 w + lane / 8
   auto swz = [](int r) { return 2 * (r & 3) + 8 * ((r >> 3) & 1); };
-  f32x4 acc[2][FB];
+  uint32_t vw[kDxLoads], vx[kXLoads];
+  const int lr = (wave * 64 + lane) / (kDxD / 8);
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int j = 0; j < kDxLoads; ++j)
+    vw[j] = 2 * ((kDxRows * j + lr) * (uint32_t)p.ldw + min(8 * (lane % (kDxD / 8) ^ swz(kDxRows * j + lr)), p.D - 8 - d0));
+#pragma unroll
+  for (int j = 0; j < kXLoads; ++j) {
+    const int m = 32 * j + 8 * wave + (lane >> 3);
+    vx[j] = 2 * (min(m, p.M - 1) * 2 * (uint32_t)p.Fp + 8 * ((lane & 7) ^ (m & 7)));
+  }
+  auto load = [&](int b, bf16* img) {
+    const int h = b >= nb, f0 = (b - h * nb) * kDxF;
+    const bf16 *w = p.w[h] + (int64_t)f0 * p.ldw + d0, *x = p.dgu + h * p.Fp + f0;
+#pragma unroll
+    for (int j = 0; j < kDxLoads; ++j) {
+      bf16* to = img + 2048 * j + 512 * wave;
+      if (f0 + kDxF <= p.F || f0 + kDxRows * j + lr < p.F) to_image(w, vw[j], to);
+      else to_image(reinterpret_cast<const bf16*>(tile::kZero16), 0, to);
+    }
+#pragma unroll
+    for (int j = 0; j < kXLoads; ++j)
+      if (FB > 1 || wave < 2) to_image(x, vx[j], img + kW + (32 * j + 8 * wave) * kDxF);
+  };
+
+  f32x4 acc[kDxI][FB];
+#pragma unroll
+  for (int i = 0; i < kDxI; ++i)
 #pragma unroll
     for (int j = 0; j < FB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const bf16* row[FB];  // of dG | dU
+  // a lane reads 4 columns of rows 8 g + r16 / 4 and 4 further
+  int wat[kDxI];
 #pragma unroll
-  for (int j = 0; j < FB; ++j) row[j] = p.dgu + (int64_t)min(16 * j + r16, p.M - 1) * 2 * p.Fp;
-
-  for (int b = b0; b < b1; ++b) {
-    const int h = b >= nb, f0 = (b - h * nb) * kDxF;
-    const bf16* w = p.w[h] + (int64_t)f0 * p.ldw;
-#pragma unroll
-    for (int j = 0; j < kDxF / 16; ++j) {
-      const int r = 16 * j + lr;
-      const int c = min(d0 + 8 * ((lane & 15) ^ swz(r)), p.D - 8);  // columns past the end: the last ones again
-      const char* s = reinterpret_cast<const char*>(w + (int64_t)r * p.ldw + c);
-      if (f0 + r >= p.F) s = reinterpret_cast<const char*>(tile::kZero16);
-      __builtin_amdgcn_global_load_lds((tile::gvoid*)s, (tile::lvoid*)(lds + (16 * j + 4 * wave) * kDxD), 16, 0, 0);
-    }
-    bf16x8 x[kDxF / 32][FB];
-#pragma unroll
-    for (int k = 0; k < kDxF / 32; ++k) {
-      const int f = f0 + 32 * k + 8 * g;
-#pragma unroll
-      for (int j = 0; j < FB; ++j) {
-        x[k][j] = load8(row[j] + h * p.Fp + min(f, p.Fp - 8));
-        if (f >= p.Fp) x[k][j] = bf16x8{};
-      }
-    }
-    __syncthreads();  // the block has landed (every wave waits for its loads before the barrier)
+  for (int i = 0; i < kDxI; ++i) {
+    const int c = 16 * (kDxI * wave + i) + 4 * (r16 & 3), r = 8 * g + (r16 >> 2);
+    wat[i] = r * kDxD + (((c >> 3) ^ swz(r)) << 3) + (c & 7);
+  }
+  for (int t = 0; t < min(n, kAhead); ++t) load(blockIdx.y + t * S, lds + t * (kW + kX));
+  int at = 0;  // block b's image
+  for (int t = 0; t < n; ++t) {
+    const bf16* img = lds + at * (kW + kX);
+    // block b is there, and every wave has read block b - 1 (a block whose rows end issues more
+    // loads than these, in which case the wait is for more than block b)
+    if (t + 1 < n) tile::vm_wait<kDxLoads + FB / 2>();
+    else tile::vm_wait<0>();
+    tile::barrier_raw();
+    at = at == kAhead ? 0 : at + 1;
+    if (t + kAhead < n) load(blockIdx.y + (t + kAhead) * S, lds + (at + kAhead - 1) % (kAhead + 1) * (kW + kX));
 #pragma unroll
     for (int k = 0; k < kDxF / 32; ++k) {
+      bf16x8 x[FB];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int c = 32 * wave + 16 * i + 4 * (r16 & 3);  // this lane's 4 columns of the rows that it reads for
-        bf16x4 q[2];
+      for (int j = 0; j < FB; ++j) x[j] = load8(img + kW + (16 * j + r16) * kDxF + (((4 * k + g) ^ (r16 & 7)) << 3));
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int r = 32 * k + 8 * g + 4 * t + (r16 >> 2);
-          q[t] = tr4(lds + r * kDxD + (((c >> 3) ^ swz(r)) << 3) + (c & 7));
-        }
-        const bf16x8 a = __builtin_shufflevector(q[0], q[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      for (int i = 0; i < kDxI; i += 2) {
+        bf16x8 a[2];
+        k == 0 ? weights<0>(a, img + wat[i], img + wat[i + 1]) : weights<2 * 32 * kDxD>(a, img + wat[i], img + wat[i + 1]);
 #pragma unroll
-        for (int j = 0; j < FB; ++j) acc[i][j] = mma(acc[i][j], a, x[k][j]);
+        for (int j = 0; j < FB; ++j) acc[i][j] = mma(acc[i][j], a[0], x[j]);
+#pragma unroll
+        for (int j = 0; j < FB; ++j) acc[i + 1][j] = mma(acc[i + 1][j], a[1], x[j]);
       }
     }
-    __syncthreads();  // read by all
   }
   // lane (r16, g): columns 4 g .. of fragment i, row r16 of group j
   float* out = p.part + (int64_t)blockIdx.y * p.M * p.D;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int d = d0 + 32 * wave + 16 * i + 4 * g;
+  for (int i = 0; i < kDxI; ++i) {
+    const int d = d0 + 16 * (kDxI * wave + i) + 4 * g;
     if (d >= p.D) continue;  // (D is a multiple of 8)
 #pragma unroll
     for (int j = 0; j < FB; ++j) {
@@ -371,12 +424,13 @@ How how_of(int64_t arows, int64_t brows, int64_t kbytes) {
 // dX from the weights as they are: for few rows, whole aligned pieces
 bool dx_rows_fit(const GatedBwdParams& p) {
   const auto a = reinterpret_cast<uintptr_t>(p.wg) | reinterpret_cast<uintptr_t>(p.wu);
-  return p.M <= 128 && p.D % 8 == 0 && p.ldw % 8 == 0 && a % 16 == 0;
+  return p.M <= 128 && p.D % 8 == 0 && p.ldw % 8 == 0 && p.ldw < (1 << 24) && a % 16 == 0;
 }
-// its K splits: two workgroups a CU, at least two blocks each (60 rows, weights of
-// 2 x 4096 x 4096: in 8 splits 32 us, 16 22, 32 26; of 2 x 4096 x 1024: 30, 17, 11)
+// its K splits: about one workgroup a CU, at least two blocks each (71 rows,
+// weights of 2 x 11520 x 3392: 46.8 us at one workgroup, 48.3 at two, 52.4 at four,
+// and the partial sums' bytes grow with the splits)
 int dx_rows_splits(int D, int F) {
-  return std::max(1, std::min(cdiv(F, kDxF), cdiv(2 * tile::kCus, cdiv(D, kDxD))));
+  return std::max(1, std::min(cdiv(F, kDxF), tile::kCus / cdiv(D, kDxD)));
 }
 
 struct Plan {
@@ -487,10 +541,8 @@ void gated_backward(const GatedBwdParams& p, hipStream_t s) {
     hipLaunchKernelGGL((gated_prepare_kernel<decltype(k)::v>), grid, dim3(256), 0, s, t);
   });
   if (rows) {
-    const int blocks = 2 * cdiv(p.F, kDxF);
-    DxRows d{{static_cast<const bf16*>(p.wg), static_cast<const bf16*>(p.wu)}, p.ldw, dgu, p.M, p.D, p.F, q.Fp,
-             cdiv(blocks, q.rows), part};
-    const int S = cdiv(blocks, d.per);
+    const DxRows d{{static_cast<const bf16*>(p.wg), static_cast<const bf16*>(p.wu)}, p.ldw, dgu, p.M, p.D, p.F, q.Fp, part};
+    const int S = q.rows;
     const dim3 g((unsigned)cdiv(p.D, kDxD), (unsigned)S);
     if (p.M <= 16) hipLaunchKernelGGL(gated_dx_rows_kernel<1>, g, dim3(256), 0, s, d);
     else if (p.M <= 32) hipLaunchKernelGGL(gated_dx_rows_kernel<2>, g, dim3(256), 0, s, d);
