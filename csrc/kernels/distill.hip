@@ -16,6 +16,10 @@
 // would leave most of the chip idle, are cut into chunks: one launch leaves
 // every chunk's maximum and sum, a second joins them and writes the gradient,
 // reading the logits again (distill_stat_kernel, distill_chunk_kernel).
+//
+// Bound by memory: 4096 x 120000 bf16 404 us, 1.97 GB at 4.9 TB/s (with stores past
+// the caches 424); 640 x 1000 fp32 6.4 us, a row's way in, two reductions and the
+// way out.
 #include "feedforward.h"
 #include "mcc/common.h"
 #include "mfma.h"

@@ -3,7 +3,7 @@
 // lane (r, g) = (lane & 15, lane >> 4) holds 16 bytes of row r, 64 bytes of K a
 // fragment, and ends with A rows 4g .. 4g+3 of B row r.
 //
-// With up to 64 B rows every byte of A is used for at most 64 products, so the
+// With up to 32 B rows every byte of A is used for at most 32 products, so the
 // weights' stream from memory is what counts.  A workgroup owns 16 A rows (of
 // each matrix when GATED) and its NW waves take the 128-byte blocks of K in
 // turn: each wave goes straight from memory into MFMA fragments with U blocks

@@ -7,6 +7,9 @@
 // round; Q = rint(S W * 127 / max |S W|) needs no 1 / rms at all.
 // Statistics are fp32.  max is taken on the bits of |S W|, which order like the
 // values with the infinities and NaN on top, so neither gets lost.
+//
+// Bound by memory: 16384 x 4096 bf16 with a residual 86 us, 470 MB at 5.5 TB/s; one
+// row of 4096 3.4 us, the row's way in, two barriers and the way out.
 #include "feedforward.h"
 #include "mcc/common.h"
 #include "mfma.h"

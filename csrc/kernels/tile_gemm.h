@@ -15,7 +15,7 @@
 // step around the 16 x 16 integer form).
 //
 // Workgroup: 4 waves in 2 x 2, wave tile (32 FA) x (32 FB), workgroup tile
-// (64 FA) x (64 FB).  Operands go HBM -> LDS by global_load_lds (16 bytes a
+// (64 FA) x (64 FB).  Operands go HBM -> LDS by buffer loads (16 bytes a
 // lane) into NST images of KS bytes of K, image kt + NST into the place of image
 // kt; how reads, loads and waits are dealt out among a step's MFMAs stands at
 // `step` below.
@@ -24,6 +24,11 @@
 // four waves read 128 KiB of LDS (1024 cycles at 128 B a cycle) and 64 KiB are
 // written: the matrix unit is the longer side.  Eight waves of half the tile
 // would read 192 KiB and be bound by LDS.
+//
+// Measured, 256 x 256 tiles over 8192 x 24576 x 4096 for half a second: bf16 1.50
+// PFLOP/s, int8 2.78 Pop/s; a library's bf16 product of that size 1.59.  The matrix
+// unit is busy 85 % of the cycles, and the clock, 1.63 GHz then, gives way to power:
+// with operands of zeros the same loop does 2.1 PFLOP/s and 4.0 Pop/s.
 //
 // An LDS row of an image is KS bytes = KS/16 slots; slot s of row r holds the
 // row's piece s ^ swz(r), applied on the source address of the load, so that
