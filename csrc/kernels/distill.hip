@@ -420,6 +420,7 @@ template <class TZ, class TG> void launch(const DistillParams& p, hipStream_t s)
   if (chunked(p.M, p.N, f32)) {
     const int n = chunks_of(p.N);
     float2* stat = static_cast<float2*>(p.work);
+    MCC_CHECK(launchable(p.M, 256, n), "distill_kl: too many rows");
     const dim3 grid((unsigned)p.M, (unsigned)n);
     hipLaunchKernelGGL(distill_stat_kernel<TZ>, grid, dim3(256), 0, s, p, stat);
     hipLaunchKernelGGL((distill_chunk_kernel<TZ, TG>), p.dz ? grid : dim3((unsigned)p.M), dim3(256),
@@ -427,6 +428,7 @@ template <class TZ, class TG> void launch(const DistillParams& p, hipStream_t s)
     return;
   }
   const int n = p.N + 7;
+  MCC_CHECK(launchable(n <= 64 * 8 * 2 ? ceil_div(p.M, 4) : p.M, n <= 256 * 8 * 4 ? 256 : 1024), "distill_kl: too many rows");
   auto rows = [&](int per) { return dim3((unsigned)ceil_div(p.M, per)); };
   const int ent = entries_bytes(p.K);
   if (n <= 64 * 8 * 2) hipLaunchKernelGGL((distill_row_kernel<TZ, TG, 64, 2>), rows(4), dim3(256), 4 * ent, s, p);
@@ -446,7 +448,7 @@ int64_t distill_bytes(int M, int N, bool z_f32) {
 
 void distill_kl(const DistillParams& p, hipStream_t s) {
   MCC_CHECK(p.M >= 0 && p.N > 0 && p.K >= 0, "distill_kl: empty rows");
-  MCC_CHECK(p.N < (1 << 30), "distill_kl: too many classes");
+  MCC_CHECK(p.N <= (1 << 30) - (1 << 16), "distill_kl: too many classes");  // (65532 chunks)
   MCC_CHECK(p.K <= kDistillMaxK, "distill_kl: too many entries per row");
   MCC_CHECK(p.ldz >= p.N, "distill_kl: row pitch");
   MCC_CHECK(p.temperature >= 0.99e-6f && p.temperature <= 1.01e6f, "distill_kl: temperature out of range");

@@ -10,6 +10,12 @@
 namespace mcc {
 namespace gpu {
 
+// whether a grid of x by y workgroups can be launched: fewer than 2^32 threads
+// along x
+inline bool launchable(int64_t x, int threads, int64_t y = 1) {
+  return x * threads < ((int64_t)1 << 32) && y <= 65535;
+}
+
 // activations of a gated block (0..2 as ActKind)
 enum GateAct : int { GATE_NONE = 0, GATE_RELU = 1, GATE_TANH = 2, GATE_SILU = 3, GATE_GELU = 4 };
 
@@ -82,7 +88,8 @@ void linear_i8(const LinearI8Params& p, hipStream_t s);
 // X, R [M][D] with pitches ldx, ldr, W [D], all bf16 or all fp32; sum [M][D]
 // contiguous in their type (written when R is given), Q int8 [M][D]
 // contiguous.  A row of zeros has scale 0; a row with a value that is not
-// finite, or whose sum of squares is not, has scale NaN and zeros in Q.
+// finite, or whose sum of squares is not (or is 0 with eps = 0 where values are
+// not), has scale NaN and zeros in Q.
 struct RmsnormI8Params {
   int M = 0, D = 0;
   bool f32 = false;

@@ -121,7 +121,9 @@ constexpr tile::Form kForms[] = {{64, 64, 2, 0.27f, 0.67f, 1.6f}, {64, 128, 2, 0
 
 template <int FA, int FB, int NST, int WPE, int ACT>
 void launch_tiles(const GatedParams& p, const Operands& o, hipStream_t s) {
-  const dim3 grid((unsigned)(cdiv(p.F, 32 * FA) * cdiv(p.M, 64 * FB)));
+  const int64_t n = (int64_t)cdiv(p.F, 32 * FA) * cdiv(p.M, 64 * FB);
+  MCC_CHECK(launchable(n, tile::kThreads), "gated_linear: too many rows");
+  const dim3 grid((unsigned)n);
   hipLaunchKernelGGL((gated_tile_kernel<FA, FB, 128, NST, WPE, ACT>), grid, dim3(tile::kThreads), 0, s, p, o);
 }
 
@@ -129,6 +131,7 @@ void launch_tiles(const GatedParams& p, const Operands& o, hipStream_t s) {
 
 void gated_forward(const GatedParams& p, hipStream_t s) {
   MCC_CHECK(p.M >= 0 && p.D > 0 && p.F > 0, "gated_linear: empty problem");
+  MCC_CHECK(p.M <= (1 << 30) && p.F <= (1 << 30), "gated_linear: too many rows");
   MCC_CHECK(p.act >= GATE_NONE && p.act <= GATE_GELU, "gated_linear: unknown activation");
   MCC_CHECK(p.ldx >= round_up(p.D, 8) && p.ldw >= round_up(p.D, 8) && p.ldx % 8 == 0 && p.ldw % 8 == 0,
             "gated_linear: row pitches must be multiples of 8");
@@ -145,7 +148,8 @@ void gated_forward(const GatedParams& p, hipStream_t s) {
   const int form = tile::best_form(kForms, p.F, p.M, steps);
   const float tiles = tile::form_us(kForms[form], tile::workgroups(kForms[form], p.F, p.M), steps);
   const float rows1 = tile::few_rows_us(true, 1, n1) * (float)steps;
-  if (p.M <= 16 || (p.M <= 32 ? rows1 <= tile::few_rows_us(true, 2, n2) * (float)steps : rows1 < tiles)) {
+  if (p.M <= 16 || (p.M <= 32 ? rows1 <= tile::few_rows_us(true, 2, n2) * (float)steps
+                                   : rows1 < tiles && cdiv(p.M, 16) <= 65535)) {
     const dim3 grid((unsigned)cdiv(p.F, 16), (unsigned)cdiv(p.M, 16));
     if (o.kbytes >= 4096) hipLaunchKernelGGL((gated_rows_kernel<1, 4, 8>), grid, dim3(512), 0, s, p, o);
     else hipLaunchKernelGGL((gated_rows_kernel<1, 4, 4>), grid, dim3(256), 0, s, p, o);

@@ -467,7 +467,9 @@ Plan plan_of(int M, int D, int F) {
 
 template <int FA, int FB, int NST, int WPE, class TO>
 void launch_tiles(const Operands& o, TO* out, int steps, int S, hipStream_t s) {
-  const dim3 grid((unsigned)(cdiv(o.arows, 64 * FA) * cdiv(o.brows, 64 * FB)), (unsigned)S);
+  const int64_t n = (int64_t)cdiv(o.arows, 64 * FA) * cdiv(o.brows, 64 * FB);
+  MCC_CHECK(launchable(n, tile::kThreads), "gated_linear_bwd: too many rows");
+  const dim3 grid((unsigned)n, (unsigned)S);
   hipLaunchKernelGGL((tile_store_kernel<FA, FB, 128, NST, WPE, TO>), grid, dim3(tile::kThreads), 0, s, o, out, steps);
 }
 template <class TO> void launch_form(int form, const Operands& o, TO* out, int steps, int S, hipStream_t s) {
@@ -536,6 +538,7 @@ void gated_backward(const GatedBwdParams& p, hipStream_t s) {
   t.rows_pad[1] = t.rows_pad[2] = q.Fp;
   t.tiles[0] = tiles(p.M, p.D);
   t.tiles[1] = t.tiles[2] = rows ? 0 : tiles(p.F, p.D);
+  MCC_CHECK(launchable((int64_t)t.tiles_g + t.tiles[0] + t.tiles[1] + t.tiles[2], 256), "gated_linear_bwd: too many rows");
   const dim3 grid((unsigned)(t.tiles_g + t.tiles[0] + t.tiles[1] + t.tiles[2]));
   with_gate(p.act, [&](auto k) {
     hipLaunchKernelGGL((gated_prepare_kernel<decltype(k)::v>), grid, dim3(256), 0, s, t);

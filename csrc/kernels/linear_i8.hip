@@ -105,7 +105,9 @@ __global__ void __launch_bounds__(64 * NW) i8_rows_kernel(LinearI8Params p, Oper
 
 template <int FA, int FB, int KS, int NST, int WPE, class TO>
 void launch_tiles(const LinearI8Params& p, const Operands& o, hipStream_t s) {
-  const dim3 grid((unsigned)(cdiv(p.N, 64 * FA) * cdiv(p.M, 64 * FB)));
+  const int64_t n = (int64_t)cdiv(p.N, 64 * FA) * cdiv(p.M, 64 * FB);
+  MCC_CHECK(launchable(n, tile::kThreads), "linear_i8: too many rows");
+  const dim3 grid((unsigned)n);
   if (p.act == ACT_RELU)
     hipLaunchKernelGGL((i8_tile_kernel<FA, FB, KS, NST, WPE, ACT_RELU, TO>), grid, dim3(tile::kThreads), 0, s, p, o);
   else if (p.act == ACT_TANH)
@@ -137,7 +139,8 @@ template <class TO> void launch(const LinearI8Params& p, hipStream_t s) {
   const int form = tile::best_form(kForms, p.N, p.M, steps);
   const float tiles = tile::form_us(kForms[form], tile::workgroups(kForms[form], p.N, p.M), steps);
   const float rows1 = tile::few_rows_us(false, 1, n1) * (float)steps;
-  if (p.M <= 16 || (p.M <= 32 ? rows1 <= tile::few_rows_us(false, 2, n2) * (float)steps : rows1 < tiles)) {
+  if (p.M <= 16 || (p.M <= 32 ? rows1 <= tile::few_rows_us(false, 2, n2) * (float)steps
+                                   : rows1 < tiles && cdiv(p.M, 16) <= 65535)) {
     const dim3 grid((unsigned)cdiv(p.N, 16), (unsigned)cdiv(p.M, 16));
     if (o.kbytes >= 4096) hipLaunchKernelGGL((i8_rows_kernel<1, 4, 8, TO>), grid, dim3(512), 0, s, p, o);
     else hipLaunchKernelGGL((i8_rows_kernel<1, 4, 4, TO>), grid, dim3(256), 0, s, p, o);
@@ -158,6 +161,7 @@ template <class TO> void launch(const LinearI8Params& p, hipStream_t s) {
 
 void linear_i8(const LinearI8Params& p, hipStream_t s) {
   MCC_CHECK(p.M >= 0 && p.N > 0 && p.K > 0, "linear_i8: empty problem");
+  MCC_CHECK(p.M <= (1 << 30) && p.N <= (1 << 30), "linear_i8: too many rows");
   MCC_CHECK(p.K <= kLinearI8MaxK, "linear_i8: K too large for an exact 32-bit sum");
   MCC_CHECK(p.act >= ACT_NONE && p.act <= ACT_TANH, "linear_i8: unknown activation");
   MCC_CHECK(p.ldx >= round_up(p.K, 16) && p.ldw >= round_up(p.K, 16) && p.ldx % 16 == 0 && p.ldw % 16 == 0,

@@ -112,15 +112,14 @@ __global__ void __launch_bounds__(RT < 256 ? 256 : RT) rmsnorm_i8_kernel(Rmsnorm
     }
   }
   if (!live) return;
-  const bool good = ss < __builtin_inff() && mx < kInfBits;
+  // (with eps = 0 rstd is infinite for a row of zeros, or whose squares underflow)
+  const float rstd = 1.f / sqrtf(ss / (float)D + p.eps);
+  const bool good = ss < __builtin_inff() && mx < kInfBits && (mx == 0 || rstd < __builtin_inff());
   const float top = ubits(mx);
   // (127 / top overflows below 2^-121: such a row is scaled in two steps)
   const float up = top < 0x1p-100f ? 0x1p100f : 1.f;
   const float inv = good && mx ? 127.f / (top * up) : 0.f;
-  if (t == 0) {
-    const float rstd = 1.f / sqrtf(ss / (float)D + p.eps);
-    p.scale[m] = good ? top * rstd / 127.f : __builtin_nanf("");
-  }
+  if (t == 0) p.scale[m] = !good ? __builtin_nanf("") : mx ? top * rstd / 127.f : 0.f;
   int8_t* q = p.q + m * D;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -147,7 +146,9 @@ __global__ void __launch_bounds__(RT < 256 ? 256 : RT) rmsnorm_i8_kernel(Rmsnorm
 
 template <class T, int RT, int NV> void launch(const RmsnormI8Params& p, bool wide, hipStream_t s) {
   constexpr int kBlock = RT < 256 ? 256 : RT;
-  const dim3 grid((unsigned)ceil_div(p.M, kBlock / RT));
+  const int64_t n = ceil_div(p.M, kBlock / RT);
+  MCC_CHECK(launchable(n, kBlock), "rmsnorm_i8: too many rows");
+  const dim3 grid((unsigned)n);
   if (wide) hipLaunchKernelGGL((rmsnorm_i8_kernel<T, RT, NV, true>), grid, dim3(kBlock), 0, s, p);
   else hipLaunchKernelGGL((rmsnorm_i8_kernel<T, RT, NV, false>), grid, dim3(kBlock), 0, s, p);
 }

@@ -69,7 +69,7 @@ def _pieces(dev, n, *ts):
         ld, unit = t.stride()
         if rows <= 1:
             ld = cols
-        if cols % n == 0 and unit == 1 and ld >= cols and ld % n == 0 and t.data_ptr() % 16 == 0:
+        if cols % n == 0 and unit == 1 and cols <= ld < 1 << 22 and ld % n == 0 and t.data_ptr() % 16 == 0:
             out.append((t, ld))
             continue
         if unit != 1 and cols > 1:
@@ -209,8 +209,8 @@ def rmsnorm_i8(x: torch.Tensor, w: torch.Tensor, residual: torch.Tensor | None =
     x, residual [M, D], w [D], all bf16 or all fp32, D <= 32768.  scale [M] fp32 = max|y| / 127 and q [M, D] int8 =
     y / scale rounded to nearest even: linear_i8's x and x_scale.  s [M, D] in x's type, from which the norm is NOT
     taken again (it is of the unrounded sum); without a residual s is x.  A row of zeros has scale 0; a row that holds
-    a value that is not finite, or overflows the fp32 sum of squares, has scale NaN and q = 0, so what is computed
-    from it is NaN.  Inference only: an 8-bit output has no gradient."""
+    a value that is not finite, or overflows the fp32 sum of squares (with eps = 0: or underflows it), has scale NaN
+    and q = 0, so what is computed from it is NaN.  Inference only: an 8-bit output has no gradient."""
     if not isinstance(x, torch.Tensor) or x.dtype not in (torch.bfloat16, torch.float32):
         _fail("x must be a bf16 or fp32 tensor")
     M, D = _matrix(x, "x", x.dtype)
@@ -219,8 +219,8 @@ def rmsnorm_i8(x: torch.Tensor, w: torch.Tensor, residual: torch.Tensor | None =
     _vector(w, "w", D, x.dtype)
     if residual is not None:
         _matrix(residual, "residual", x.dtype, M, D)
-    if not eps >= 0:
-        _fail(f"rmsnorm_i8: eps = {eps} must not be negative")
+    if not 0 <= eps < 1e38:
+        _fail(f"rmsnorm_i8: eps = {eps} must be finite and not negative")
     dev = _device(x, w, residual)
     q = torch.empty(M, D, dtype=torch.int8, device=dev)
     scale = torch.empty(M, dtype=torch.float32, device=dev)

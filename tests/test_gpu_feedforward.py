@@ -584,6 +584,78 @@ def test_empty_batches(cuda):
     assert dz.shape == (0, 64) and loss.shape == (0,)
 
 
+@pytest.mark.gpu
+def test_rmsnorm_i8_without_eps(cuda):
+    """eps = 0: a row of zeros has scale 0, a row whose squares underflow is NaN, others are as they were."""
+    g = gen(5, cuda)
+    x, w = randn(g, 6, 320, dtype=torch.float32), randn(g, 320, dtype=torch.float32)
+    x[1] = 0
+    x[3] *= 1e-30
+    q, scale, _ = ops.rmsnorm_i8(x, w, eps=0.0)
+    assert scale[1].item() == 0 and not q[1].any()
+    assert math.isnan(scale[3].item()) and not q[3].any()
+    rows = [0, 2, 4, 5]
+    v = x[rows]
+    norm_check(v, w, None, 0.0, (q[rows], scale[rows], v))
+
+
+@pytest.mark.gpu
+def test_many_short_rows(cuda):
+    """More rows than 65535 groups of 16."""
+    g = gen(6, cuda)
+    M = 1_100_003
+    case = gated_bwd_case(g, M, 24, 8)
+    gated_check(*case[1:4], "silu", ops.gated_linear(*case[1:4], "silu", save=True), True)
+    gated_bwd_check(*case, "silu", ops.gated_linear_bwd(*case, "silu"))
+    x, sx, w, sw, b = i8_case(g, M, 7, 40)
+    i8_check(x, sx, w, sw, b, "relu", ops.linear_i8(x, sx, w, sw, b, "relu"))
+    x, w = randn(g, M, 10), randn(g, 10)
+    norm_check(x, w, x, 1e-6, ops.rmsnorm_i8(x, w, x))
+    z, tv, ti = distill_case(g, M, 5, 2)
+    distill_check(z, tv, ti, 1.0, 1.0, *ops.distill_kl(z, tv, ti))
+
+
+def spread(M, cuda):
+    """Rows of a large matrix, the first and the last among them."""
+    return torch.tensor([0, 1, M // 3, M // 2, M - 130, M - 2, M - 1], device=cuda)
+
+
+@pytest.mark.gpu
+def test_matrices_past_32_bits(cuda):
+    """Matrices of more than 2^31 values: what rows far behind hold."""
+    g = gen(7, cuda)
+    M, F, D = 70_001, 32_768, 8
+    at = spread(M, cuda)
+    x, wg, wu = randn(g, M, D), randn(g, F, D), randn(g, F, D)
+    h, gate, up = ops.gated_linear(x, wg, wu, "silu", save=True)
+    gated_check(x[at], wg, wu, "silu", (h[at], gate[at], up[at]), True)
+    # gradients of these rows alone, the others' are zeros
+    h.zero_()
+    h[at] = randn(g, at.numel(), F, std=0.1)
+    dx, dwg, dwu = ops.gated_linear_bwd(h, x, wg, wu, gate, up, "silu")
+    gated_bwd_check(h[at], x[at], wg, wu, gate[at], up[at], "silu", (dx[at], dwg, dwu))
+    dx[at] = 0
+    assert not dx.any()
+    del h, gate, up, dx, dwg, dwu
+    F = F + 1  # (rows of any alignment)
+    x, sx, w, sw, b = i8_case(g, M, F, 16)
+    i8_check(x[at], sx[at], w, sw, b, "none", ops.linear_i8(x, sx, w, sw, b)[at])
+
+
+@pytest.mark.gpu
+def test_rows_past_32_bits(cuda):
+    g = gen(8, cuda)
+    M, D = 70_001, 32_767
+    at = spread(M, cuda)
+    x, w = randn(g, M, D), randn(g, D)
+    q, scale, s = ops.rmsnorm_i8(x, w, x)
+    norm_check(x[at], w, x[at], 1e-6, (q[at], scale[at], s[at]))
+    del q, scale, s
+    _, tv, ti = distill_case(g, M, 50, 3)
+    dz, loss = ops.distill_kl(x, tv, ti)
+    distill_check(x[at], tv[at], ti[at], 1.0, 1.0, dz[at], loss[at])
+
+
 def serving(x, r, w, w1, s1, b1):
     """A quantised projection behind its norm."""
     q, s, v = ops.rmsnorm_i8(x, w, r)
@@ -737,6 +809,7 @@ def test_refusals():
     refused("residual has shape", ops.rmsnorm_i8, x, x[0], h)
     refused("eps", ops.rmsnorm_i8, x, x[0], eps=-1.0)
     refused("eps", ops.rmsnorm_i8, x, x[0], eps=float("nan"))
+    refused("eps", ops.rmsnorm_i8, x, x[0], eps=float("inf"))
     refused("rows of 1 to 32768", ops.rmsnorm_i8, torch.zeros(1, 32769), torch.zeros(32769))
     refused("on the GPU", ops.rmsnorm_i8, x, x[0])
     t, i = torch.zeros(4, 3), torch.zeros(4, 3, dtype=torch.int64)
