@@ -21,7 +21,7 @@ enum GateAct : int { GATE_NONE = 0, GATE_RELU = 1, GATE_TANH = 2, GATE_SILU = 3,
 
 // H = f(X Wg^T) * (X Wu^T), bf16.  X [M][ldx], Wg / Wu [F][ldw], H / G / U
 // [M][F] contiguous; ldx, ldw multiples of 8, X, Wg, Wu 16-byte aligned, and
-// columns D .. round_up(D, 8) of their rows readable and zero.  gate / up
+// columns D .. round_up(D, 8) of their rows readable and zero, unless `any`.  gate / up
 // (both or neither): the two projections, kept for the backward pass.
 struct GatedParams {
   int M = 0, D = 0, F = 0, act = GATE_SILU;
@@ -32,7 +32,9 @@ struct GatedParams {
   void* h = nullptr;
   void* gate = nullptr;
   void* up = nullptr;
+  bool any = false;  // up to kAnyRows rows of X: rows of any pitch, length and 2-byte alignment
 };
+constexpr int kAnyRows = 32;
 void gated_forward(const GatedParams& p, hipStream_t s);
 
 // The backward pass of H = f(G) * U from dH [M][F] and the saved G, U [M][F]
@@ -74,6 +76,7 @@ struct LinearI8Params {
   const float* bias = nullptr;  // optional
   void* y = nullptr;
   bool f32 = false;
+  bool any = false;  // up to kAnyRows rows of X: rows of any pitch, length and alignment
 };
 // the largest K whose sum of products of two int8 cannot pass 32 bits:
 // 131071 * 128 * 128 < 2^31

@@ -28,8 +28,51 @@ inline float few_rows_us(bool two, int fb, int64_t n) {
   return us * (n < kCus ? 1.f : (float)n / kCus);
 }
 
-// NM: matrices on the A side (2: a gate and its projection)
-template <class E, int FB, int U, int NW, int NM>
+// 16 bytes from any address: the two aligned pieces that hold them (each holds a
+// byte that is wanted, so neither can lie in another page), cut together when
+// all loads are on their way
+struct Cut {
+  uint32_t lo __attribute__((ext_vector_type(4))), hi __attribute__((ext_vector_type(4)));
+  __device__ __forceinline__ void load(const char* p, int n) {  // the first n of them, n > 0
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+    lo = *reinterpret_cast<const u4*>(a & ~(uintptr_t)15);
+    hi = *reinterpret_cast<const u4*>((a + n - 1) & ~(uintptr_t)15);
+  }
+  __device__ __forceinline__ i32x4 get(int by) const {  // by = p % 16
+    typedef uint32_t u8 __attribute__((ext_vector_type(8)));
+    u8 w = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    w = by & 8 ? __builtin_shufflevector(w, w, 2, 3, 4, 5, 6, 7, 7, 7) : w;
+    w = by & 4 ? __builtin_shufflevector(w, w, 1, 2, 3, 4, 5, 6, 7, 7) : w;
+    i32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (int)__builtin_amdgcn_alignbyte(w[i + 1], w[i], by & 3);
+    return v;
+  }
+};
+// bytes o .. o + 15 of a row of n, zeros behind its end
+__device__ __forceinline__ i32x4 load_end(const char* row, int64_t o, int64_t n) {
+  const int left = (int)min(n - o, (int64_t)16);
+  i32x4 v = {0, 0, 0, 0};
+  if (left <= 0) return v;
+  Cut c;
+  c.load(row + o, left);
+  v = c.get((int)(reinterpret_cast<uintptr_t>(row + o) & 15));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int b = left - 4 * i;
+    v[i] = b >= 4 ? v[i] : b <= 0 ? 0 : v[i] & (int)(0xffffffffu >> (32 - 8 * b));
+  }
+  return v;
+}
+
+// NM: matrices on the A side (2: a gate and its projection).  ANY: rows of any
+// address, pitch and length instead of whole aligned pieces: the copy into padded
+// rows would read the weights, write them and read them again (1 x 5500 x 12370
+// int8 39 us, so 26; 32 x
+// 4095 x 8192 gated 75 and 69).  Unaligned loads, which the hardware takes, took 35 and
+// 101.
+template <class E, int FB, int U, int NW, int NM, bool ANY = false>
 struct FewRows {
   typedef typename E::frag frag;
   typedef typename E::acc acc_t;
@@ -43,9 +86,16 @@ struct FewRows {
     const char* pa[NM];
     const char* pb[FB];
 #pragma unroll
-    for (int h = 0; h < NM; ++h) pa[h] = p.a[h] + (int64_t)min(a0 + r16, p.arows - 1) * p.lda + g * 16;
+    for (int h = 0; h < NM; ++h) pa[h] = p.a[h] + (int64_t)min(a0 + r16, p.arows - 1) * p.lda + (ANY ? 0 : g * 16);
 #pragma unroll
-    for (int j = 0; j < FB; ++j) pb[j] = p.b + (int64_t)min(b0 + 16 * j + r16, p.brows - 1) * p.ldb + g * 16;
+    for (int j = 0; j < FB; ++j) pb[j] = p.b + (int64_t)min(b0 + 16 * j + r16, p.brows - 1) * p.ldb + (ANY ? 0 : g * 16);
+    int ba[NM], bb[FB];  // of a row's pieces: where they start in an aligned one
+    if constexpr (ANY) {
+#pragma unroll
+      for (int h = 0; h < NM; ++h) ba[h] = (int)(reinterpret_cast<uintptr_t>(pa[h]) & 15);
+#pragma unroll
+      for (int j = 0; j < FB; ++j) bb[j] = (int)(reinterpret_cast<uintptr_t>(pb[j]) & 15);
+    }
 
     acc_t acc[NM][FB];
 #pragma unroll
@@ -59,6 +109,35 @@ struct FewRows {
     const int64_t nfull = p.kbytes / kStep;
     int64_t blk = wave;
     for (; blk + (int64_t)(U - 1) * NW < nfull; blk += (int64_t)U * NW) {
+      if constexpr (ANY) {
+        Cut ca[U][NM][2], cb[U][FB][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int64_t o = (blk + u * NW) * kStep + 16 * g;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+#pragma unroll
+            for (int h = 0; h < NM; ++h) ca[u][h][k].load(pa[h] + o + 64 * k, 16);
+#pragma unroll
+            for (int j = 0; j < FB; ++j) cb[u][j][k].load(pb[j] + o + 64 * k, 16);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            frag xb[FB];
+#pragma unroll
+            for (int j = 0; j < FB; ++j) xb[j] = __builtin_bit_cast(frag, cb[u][j][k].get(bb[j]));
+#pragma unroll
+            for (int h = 0; h < NM; ++h) {
+              const frag xa = __builtin_bit_cast(frag, ca[u][h][k].get(ba[h]));
+#pragma unroll
+              for (int j = 0; j < FB; ++j) acc[h][j] = E::mul(xa, xb[j], acc[h][j]);
+            }
+          }
+        continue;
+      }
       frag xa[U][NM][2], xb[U][FB][2];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -87,16 +166,17 @@ struct FewRows {
         const int64_t o = blk * kStep + 64 * k;
         const bool in = o + g * 16 < p.kbytes;
         const frag z = __builtin_bit_cast(frag, i32x4{0, 0, 0, 0});
+        auto last = [&](const char* row) {
+          if constexpr (ANY) return __builtin_bit_cast(frag, load_end(row, o + g * 16, p.kbytes));
+          const frag v = *reinterpret_cast<const frag*>(row + (in ? o : -(int64_t)(g * 16)));
+          return in ? v : z;
+        };
         frag xb[FB];
 #pragma unroll
-        for (int j = 0; j < FB; ++j) {
-          xb[j] = *reinterpret_cast<const frag*>(pb[j] + (in ? o : -(int64_t)(g * 16)));
-          if (!in) xb[j] = z;
-        }
+        for (int j = 0; j < FB; ++j) xb[j] = last(pb[j]);
 #pragma unroll
         for (int h = 0; h < NM; ++h) {
-          frag xa = *reinterpret_cast<const frag*>(pa[h] + (in ? o : -(int64_t)(g * 16)));
-          if (!in) xa = z;
+          const frag xa = last(pa[h]);
 #pragma unroll
           for (int j = 0; j < FB; ++j) acc[h][j] = E::mul(xa, xb[j], acc[h][j]);
         }

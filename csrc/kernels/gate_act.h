@@ -23,9 +23,20 @@ __device__ __forceinline__ void normal(float v, float& cdf, float& bell) {
   cdf = v < 0.f ? half : 1.f - half;
 }
 
+// tanh by Lambert's continued fraction v / (1 + s / (3 + s / (5 + s / (7 + s / 9)))),
+// s = v^2, where 1 - 2 / (exp(2 |v|) + 1) would lose digits; off by up to 5 units
+// of 2^-24.  With the library's tanhf 1481 x 64 x 9233 took 63.5 us (relu: 37), so 50.
+__device__ __forceinline__ float tanh_(float v) {
+  const float a = fabsf(v), s = v * v;
+  const bool small = a < 0.7f;
+  const float r = __builtin_amdgcn_rcpf(small ? fmaf(s, fmaf(s, 15.f, 420.f), 945.f)
+                                              : __builtin_amdgcn_exp2f(2.f * kLog2e * a) + 1.f);
+  return copysignf(small ? a * fmaf(s, s + 105.f, 945.f) * r : fmaf(-2.f, r, 1.f), v);
+}
+
 template <int A> __device__ __forceinline__ float gate_f(float v) {
   if constexpr (A == GATE_RELU) return v < 0.f ? 0.f : v;  // keeps a NaN
-  if constexpr (A == GATE_TANH) return tanhf(v);
+  if constexpr (A == GATE_TANH) return tanh_(v);
   if constexpr (A == GATE_SILU) return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * v));
   if constexpr (A == GATE_GELU) {
     float cdf, bell;
@@ -52,7 +63,7 @@ template <int A> __device__ __forceinline__ void gate_slope(float v, float& f, f
     f = gate_f<A>(v);
     d = v > 0.f ? 1.f : 0.f;
   } else if constexpr (A == GATE_TANH) {
-    f = tanhf(v);
+    f = tanh_(v);
     d = 1.f - f * f;
   } else if constexpr (A == GATE_SILU) {
     const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * v));

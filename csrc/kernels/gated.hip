@@ -39,7 +39,7 @@ Operands operands(const GatedParams& p) {
   o.ldb = p.ldx * 2;
   o.arows = p.F;
   o.brows = p.M;
-  o.kbytes = round_up(p.D, 8) * 2;
+  o.kbytes = (p.any ? p.D : round_up(p.D, 8)) * 2;
   return o;
 }
 
@@ -86,9 +86,9 @@ __global__ void __launch_bounds__(tile::kThreads, WPE) gated_tile_kernel(GatedPa
   }
 }
 
-template <int FB, int U, int NW>
+template <int FB, int U, int NW, bool ANY>
 __global__ void __launch_bounds__(64 * NW) gated_rows_kernel(GatedParams p, Operands op) {
-  typedef FewRows<Bf16, FB, U, NW, 2> R;
+  typedef FewRows<Bf16, FB, U, NW, 2, ANY> R;
   __shared__ __attribute__((aligned(16))) char lds[R::kLds];
   const int f0 = blockIdx.x * 16, m0 = blockIdx.y * R::kRows;
   R::run(op, lds, f0, m0);
@@ -133,10 +133,12 @@ void gated_forward(const GatedParams& p, hipStream_t s) {
   MCC_CHECK(p.M >= 0 && p.D > 0 && p.F > 0, "gated_linear: empty problem");
   MCC_CHECK(p.M <= (1 << 30) && p.F <= (1 << 30), "gated_linear: too many rows");
   MCC_CHECK(p.act >= GATE_NONE && p.act <= GATE_GELU, "gated_linear: unknown activation");
-  MCC_CHECK(p.ldx >= round_up(p.D, 8) && p.ldw >= round_up(p.D, 8) && p.ldx % 8 == 0 && p.ldw % 8 == 0,
+  MCC_CHECK(!p.any || p.M <= kAnyRows, "gated_linear: too many rows of any alignment");
+  MCC_CHECK(p.any || (p.ldx >= round_up(p.D, 8) && p.ldw >= round_up(p.D, 8) && p.ldx % 8 == 0 && p.ldw % 8 == 0),
             "gated_linear: row pitches must be multiples of 8");
-  MCC_CHECK(p.ldx < (1 << 22) && p.ldw < (1 << 22), "gated_linear: row pitch too large");
-  MCC_CHECK((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.wg) | reinterpret_cast<uintptr_t>(p.wu)) %
+  MCC_CHECK(p.any || (p.ldx < (1 << 22) && p.ldw < (1 << 22)), "gated_linear: row pitch too large");
+  MCC_CHECK(p.ldx >= 0 && p.ldw >= 0, "gated_linear: row pitch");
+  MCC_CHECK(p.any || (reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.wg) | reinterpret_cast<uintptr_t>(p.wu)) %
                     16 == 0, "gated_linear: operands must be 16-byte aligned");
   MCC_CHECK((p.gate == nullptr) == (p.up == nullptr), "gated_linear: gate and up go together");
   if (p.M == 0) return;
@@ -151,10 +153,15 @@ void gated_forward(const GatedParams& p, hipStream_t s) {
   if (p.M <= 16 || (p.M <= 32 ? rows1 <= tile::few_rows_us(true, 2, n2) * (float)steps
                                    : rows1 < tiles && cdiv(p.M, 16) <= 65535)) {
     const dim3 grid((unsigned)cdiv(p.F, 16), (unsigned)cdiv(p.M, 16));
-    if (o.kbytes >= 4096) hipLaunchKernelGGL((gated_rows_kernel<1, 4, 8>), grid, dim3(512), 0, s, p, o);
-    else hipLaunchKernelGGL((gated_rows_kernel<1, 4, 4>), grid, dim3(256), 0, s, p, o);
+    const bool eight = o.kbytes >= 4096;
+    if (p.any && eight) hipLaunchKernelGGL((gated_rows_kernel<1, 2, 8, true>), grid, dim3(512), 0, s, p, o);
+    else if (p.any) hipLaunchKernelGGL((gated_rows_kernel<1, 2, 4, true>), grid, dim3(256), 0, s, p, o);
+    else if (eight) hipLaunchKernelGGL((gated_rows_kernel<1, 4, 8, false>), grid, dim3(512), 0, s, p, o);
+    else hipLaunchKernelGGL((gated_rows_kernel<1, 4, 4, false>), grid, dim3(256), 0, s, p, o);
   } else if (p.M <= 32) {
-    hipLaunchKernelGGL((gated_rows_kernel<2, 2, 4>), dim3((unsigned)cdiv(p.F, 16)), dim3(256), 0, s, p, o);
+    const dim3 grid((unsigned)cdiv(p.F, 16));
+    if (p.any) hipLaunchKernelGGL((gated_rows_kernel<2, 2, 4, true>), grid, dim3(256), 0, s, p, o);
+    else hipLaunchKernelGGL((gated_rows_kernel<2, 2, 4, false>), grid, dim3(256), 0, s, p, o);
   } else {
     with_gate(p.act, [&](auto k) {
       constexpr int A = decltype(k)::v;

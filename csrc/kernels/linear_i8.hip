@@ -12,6 +12,7 @@
 // 8192 x 12288 x 4096 330 (2.5 Pop/s).
 #include "feedforward.h"
 #include "few_rows.h"
+#include "gate_act.h"
 #include "kernels.h"
 #include "mcc/common.h"
 #include "tile_gemm.h"
@@ -29,7 +30,8 @@ using tile::Tile;
 // ReLU that keeps a NaN (a row whose scale is NaN stays visible)
 template <int A> __device__ __forceinline__ float act_i8(float v) {
   if constexpr (A == ACT_RELU) return v < 0.f ? 0.f : v;
-  else return act_c<A>(v);
+  else if constexpr (A == ACT_TANH) return tanh_(v);
+  else return v;
 }
 
 template <int FA, int FB, int KS, int NST, int WPE, int ACT, class TO>
@@ -85,9 +87,9 @@ __global__ void __launch_bounds__(tile::kThreads, WPE) i8_tile_kernel(LinearI8Pa
   }
 }
 
-template <int FB, int U, int NW, class TO>
+template <int FB, int U, int NW, bool ANY, class TO>
 __global__ void __launch_bounds__(64 * NW) i8_rows_kernel(LinearI8Params p, Operands op) {
-  typedef FewRows<I8, FB, U, NW, 1> R;
+  typedef FewRows<I8, FB, U, NW, 1, ANY> R;
   __shared__ __attribute__((aligned(16))) char lds[R::kLds];
   const int n0 = blockIdx.x * 16, m0 = blockIdx.y * R::kRows;
   R::run(op, lds, n0, m0);
@@ -131,7 +133,7 @@ template <class TO> void launch(const LinearI8Params& p, hipStream_t s) {
   o.ldb = p.ldx;
   o.arows = p.N;
   o.brows = p.M;
-  o.kbytes = round_up(p.K, 16);
+  o.kbytes = p.any ? p.K : round_up(p.K, 16);
   // up to 32 rows the weights' way from memory counts, which many workgroups
   // that stream share best; above, whatever the measured step times say
   const int64_t n1 = (int64_t)cdiv(p.N, 16) * cdiv(p.M, 16), n2 = (int64_t)cdiv(p.N, 16) * cdiv(p.M, 32);
@@ -142,10 +144,15 @@ template <class TO> void launch(const LinearI8Params& p, hipStream_t s) {
   if (p.M <= 16 || (p.M <= 32 ? rows1 <= tile::few_rows_us(false, 2, n2) * (float)steps
                                    : rows1 < tiles && cdiv(p.M, 16) <= 65535)) {
     const dim3 grid((unsigned)cdiv(p.N, 16), (unsigned)cdiv(p.M, 16));
-    if (o.kbytes >= 4096) hipLaunchKernelGGL((i8_rows_kernel<1, 4, 8, TO>), grid, dim3(512), 0, s, p, o);
-    else hipLaunchKernelGGL((i8_rows_kernel<1, 4, 4, TO>), grid, dim3(256), 0, s, p, o);
+    const bool eight = o.kbytes >= 4096;
+    if (p.any && eight) hipLaunchKernelGGL((i8_rows_kernel<1, 2, 8, true, TO>), grid, dim3(512), 0, s, p, o);
+    else if (p.any) hipLaunchKernelGGL((i8_rows_kernel<1, 2, 4, true, TO>), grid, dim3(256), 0, s, p, o);
+    else if (eight) hipLaunchKernelGGL((i8_rows_kernel<1, 4, 8, false, TO>), grid, dim3(512), 0, s, p, o);
+    else hipLaunchKernelGGL((i8_rows_kernel<1, 4, 4, false, TO>), grid, dim3(256), 0, s, p, o);
   } else if (p.M <= 32) {
-    hipLaunchKernelGGL((i8_rows_kernel<2, 2, 4, TO>), dim3((unsigned)cdiv(p.N, 16)), dim3(256), 0, s, p, o);
+    const dim3 grid((unsigned)cdiv(p.N, 16));
+    if (p.any) hipLaunchKernelGGL((i8_rows_kernel<2, 2, 4, true, TO>), grid, dim3(256), 0, s, p, o);
+    else hipLaunchKernelGGL((i8_rows_kernel<2, 2, 4, false, TO>), grid, dim3(256), 0, s, p, o);
   } else {
     switch (form) {
       case 0: launch_tiles<1, 1, 128, 4, 2, TO>(p, o, s); break;
@@ -164,10 +171,12 @@ void linear_i8(const LinearI8Params& p, hipStream_t s) {
   MCC_CHECK(p.M <= (1 << 30) && p.N <= (1 << 30), "linear_i8: too many rows");
   MCC_CHECK(p.K <= kLinearI8MaxK, "linear_i8: K too large for an exact 32-bit sum");
   MCC_CHECK(p.act >= ACT_NONE && p.act <= ACT_TANH, "linear_i8: unknown activation");
-  MCC_CHECK(p.ldx >= round_up(p.K, 16) && p.ldw >= round_up(p.K, 16) && p.ldx % 16 == 0 && p.ldw % 16 == 0,
+  MCC_CHECK(!p.any || p.M <= kAnyRows, "linear_i8: too many rows of any alignment");
+  MCC_CHECK(p.ldx >= 0 && p.ldw >= 0, "linear_i8: row pitch");
+  MCC_CHECK(p.any || (p.ldx >= round_up(p.K, 16) && p.ldw >= round_up(p.K, 16) && p.ldx % 16 == 0 && p.ldw % 16 == 0),
             "linear_i8: row pitches must be multiples of 16");
-  MCC_CHECK(p.ldx < (1 << 23) && p.ldw < (1 << 23), "linear_i8: row pitch too large");
-  MCC_CHECK((reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w)) % 16 == 0,
+  MCC_CHECK(p.any || (p.ldx < (1 << 23) && p.ldw < (1 << 23)), "linear_i8: row pitch too large");
+  MCC_CHECK(p.any || (reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.w)) % 16 == 0,
             "linear_i8: operands must be 16-byte aligned");
   if (p.M == 0) return;
   if (p.f32) launch<float>(p, s);

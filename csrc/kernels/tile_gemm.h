@@ -361,41 +361,67 @@ struct RowStore {
     } else {
       // Rows that start anywhere: the 16-byte pieces of memory that lie wholly in
       // a row's run, each cut out of two slots, then the up to 15 bytes at either
-      // end by element.  (All by element, 777 x 1024 x 2731 with three outputs
-      // took 28 us; with rows of whole pieces it takes 16.)
-      constexpr int kRows = 64 / kSlots;
+      // end, an 8-, a 4- and a 2-byte store (with a store per value 777 x 1024 x
+      // 2731 with three outputs took 24.0 us, so 22.3; rows of whole pieces 18.7).
+      typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+      typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+      typedef uint32_t u8 __attribute__((ext_vector_type(8)));
+      constexpr int kRows = 64 / kSlots, kSize = (int)sizeof(TO);
       const int cols = min(32 * NF, N - n0);  // columns that exist
       if (cols <= 0) return;
+      if (cols < kVec) {
+        const int row = lane & 31;
+        TO* q = out + (int64_t)(m0 + row) * N + n0;
+        for (int c = lane >> 5; c < cols && m0 + row < M; c += 2)
+          q[c] = *reinterpret_cast<const TO*>(lds + at(row, 0) + c * kSize);
+        return;
+      }
       auto skip = [&](int row) {  // columns before the first whole piece of a row
         const uintptr_t a = reinterpret_cast<uintptr_t>(out + (int64_t)(m0 + row) * N + n0);
-        return (int)((16 - a % 16) % 16 / sizeof(TO));
+        return (int)((16 - a % 16) % 16 / kSize);
       };
-      const int slot = lane % kSlots;
-#pragma unroll 4
-      for (int t = 0; t < 32 / kRows; ++t) {
-        const int row = t * kRows + lane / kSlots, c0 = skip(row), c = c0 + slot * kVec;
-        if (m0 + row >= M || c + kVec > cols) continue;
-        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-        typedef uint32_t u8 __attribute__((ext_vector_type(8)));
-        const u4 lo = *reinterpret_cast<const u4*>(lds + at(row, slot));
-        const u4 hi = *reinterpret_cast<const u4*>(lds + at(row, c0 ? slot + 1 : slot));
-        const int by = c0 * (int)sizeof(TO);
-        // (whole vectors selected: an indexed array would be put into LDS)
+      // 16 bytes from byte `by` of lo on, into hi (whole vectors selected: an indexed array would be put into LDS)
+      auto cut = [](const u4& lo, const u4& hi, int by) {
         u8 w = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         w = by & 8 ? __builtin_shufflevector(w, w, 2, 3, 4, 5, 6, 7, 7, 7) : w;
         w = by & 4 ? __builtin_shufflevector(w, w, 1, 2, 3, 4, 5, 6, 7, 7) : w;
         u4 v;
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_alignbyte(w[i + 1], w[i], by & 2);
-        *reinterpret_cast<u4*>(out + (int64_t)(m0 + row) * N + n0 + c) = v;
+        return v;
+      };
+      const int slot = lane % kSlots;
+#pragma unroll 4
+      for (int t = 0; t < 32 / kRows; ++t) {
+        const int row = t * kRows + lane / kSlots, c0 = skip(row), c = c0 + slot * kVec;
+        if (m0 + row >= M || c + kVec > cols) continue;
+        const u4 lo = *reinterpret_cast<const u4*>(lds + at(row, slot));
+        const u4 hi = *reinterpret_cast<const u4*>(lds + at(row, c0 ? slot + 1 : slot));
+        *reinterpret_cast<u4*>(out + (int64_t)(m0 + row) * N + n0 + c) = cut(lo, hi, c0 * kSize);
       }
-      // lane = (row, end)
-      const int row = lane & 31, c0 = min(skip(row), cols);
-      const int from = lane < 32 ? 0 : c0 + (cols - c0) / kVec * kVec, to = lane < 32 ? c0 : cols;
-      if (m0 + row < M) {
-        TO* q = out + (int64_t)(m0 + row) * N + n0;
-        for (int c = from; c < to; ++c)
-          q[c] = *reinterpret_cast<const TO*>(lds + at(row, c / kVec) + (c % kVec) * (int)sizeof(TO));
+      // lane = (row, end): the piece that ends where the row's first whole one starts, or the one that
+      // starts where the last ends, of which the run has the last or the first `len` values
+      const int row = lane & 31, c0 = skip(row), n = (cols - c0) / kVec;
+      const bool head = lane < 32;
+      const int len = head ? c0 : cols - c0 - n * kVec;
+      if (m0 + row >= M || len == 0) return;
+      const int s = head ? 0 : n;  // (len > 0: a slot that exists)
+      const u4 lo = *reinterpret_cast<const u4*>(lds + at(row, s));
+      const u4 hi = *reinterpret_cast<const u4*>(lds + at(row, head ? 0 : min(s + 1, kSlots - 1)));
+      const u4 v = cut(lo, hi, c0 * kSize);
+      char* q = reinterpret_cast<char*>(out + (int64_t)(m0 + row) * N + n0 + c0 + (head ? -kVec : n * kVec));
+      const int bytes = len * kSize;
+      if (bytes & 8) *reinterpret_cast<u2*>(q + (head ? 8 : 0)) = head ? u2{v[2], v[3]} : u2{v[0], v[1]};
+      if (bytes & 4) {
+        const int d = head ? (bytes & 8 ? 1 : 3) : (bytes & 8 ? 2 : 0);
+        *reinterpret_cast<uint32_t*>(q + 4 * d) = head ? (bytes & 8 ? v[1] : v[3]) : (bytes & 8 ? v[2] : v[0]);
+      }
+      if constexpr (kSize == 2) {
+        if (len & 1) {  // value 8 - len (odd) or len - 1 (even)
+          const int i = head ? 8 - len : len - 1;
+          const uint32_t d = i & 4 ? (i & 2 ? v[3] : v[2]) : (i & 2 ? v[1] : v[0]);
+          *reinterpret_cast<uint16_t*>(q + 2 * i) = (uint16_t)(head ? d >> 16 : d);
+        }
       }
     }
   }

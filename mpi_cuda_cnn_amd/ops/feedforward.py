@@ -8,7 +8,7 @@ function of its own.
 
 Rows may be strided views.  The kernels read rows in 16-byte pieces: tensors
 whose rows are not whole pieces, or not aligned to them, are copied into padded
-rows first, in one launch a call.
+rows first, in one launch a call; products of up to 32 rows take them as they are.
 """
 
 from __future__ import annotations
@@ -61,9 +61,11 @@ def _device(first, *more):
 
 
 def _pieces(dev, n, *ts):
-    """((t or a copy, row pitch), ..): rows of whole, aligned 16-byte pieces of n elements, zeros behind the last
-    column.  All copies that a call needs are made by one kernel."""
+    """((t or a copy, row pitch), .., any): rows of whole, aligned 16-byte pieces of n elements, zeros behind the last
+    column.  All copies that a call needs are made by one kernel; none for few rows of the first (any is then True),
+    where a copy of the weights would cost more than the product."""
     out, todo = [], None
+    few = ts[0].shape[0] <= _K.ANY_ROWS
     for t in ts:
         rows, cols = t.shape
         ld, unit = t.stride()
@@ -75,6 +77,10 @@ def _pieces(dev, n, *ts):
         if unit != 1 and cols > 1:
             t = t.contiguous()
             ld = cols
+        if few:
+            out.append((t, ld))
+            todo = ()
+            continue
         pitch = (cols + n - 1) // n * n
         copy = torch.empty(rows, pitch, dtype=t.dtype, device=dev)
         size = t.element_size()
@@ -82,8 +88,9 @@ def _pieces(dev, n, *ts):
             todo = []
         todo.append((t.data_ptr(), copy.data_ptr(), ld * size, pitch * size, rows, cols * size))
         out.append((copy, pitch))
-    if todo is not None:
+    if todo:
         _run(dev, _K.pad_rows, todo)
+    out.append(todo == ())
     return out
 
 
@@ -121,11 +128,11 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act:
     h = torch.empty(M, F, dtype=torch.bfloat16, device=dev)
     gate, up = (torch.empty_like(h), torch.empty_like(h)) if save else (None, None)
     if M:
-        (xa, ldx), (wg, ldw), (wu, ldu) = _pieces(dev, 8, x, w_gate, w_up)
+        (xa, ldx), (wg, ldw), (wu, ldu), any_ = _pieces(dev, 8, x, w_gate, w_up)
         if ldu != ldw:  # both weights are read with one pitch
             wg, wu, ldw = wg.contiguous(), wu.contiguous(), wg.shape[1]
         _run(dev, _K.gated_forward, M, D, F, kind, xa.data_ptr(), ldx, wg.data_ptr(), wu.data_ptr(), ldw, h.data_ptr(),
-             gate.data_ptr() if save else 0, up.data_ptr() if save else 0)
+             gate.data_ptr() if save else 0, up.data_ptr() if save else 0, any_)
     return (h, gate, up) if save else h
 
 
@@ -153,11 +160,11 @@ def linear_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     dev = _device(x, x_scale, w, w_scale, b)
     y = torch.empty(M, N, dtype=out_dtype, device=dev)
     if M:
-        (xa, ldx), (wa, ldw) = _pieces(dev, 16, x, w)
+        (xa, ldx), (wa, ldw), any_ = _pieces(dev, 16, x, w)
         sx, sw = x_scale.contiguous(), w_scale.contiguous()
         bias = b.contiguous() if b is not None else None
         _run(dev, _K.linear_i8, M, N, K, _ACT[act], xa.data_ptr(), ldx, sx.data_ptr(), wa.data_ptr(), ldw, sw.data_ptr(),
-             bias.data_ptr() if bias is not None else 0, y.data_ptr(), out_dtype == torch.float32)
+             bias.data_ptr() if bias is not None else 0, y.data_ptr(), out_dtype == torch.float32, any_)
     return y
 
 

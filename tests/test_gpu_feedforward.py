@@ -557,6 +557,18 @@ def test_linear_i8_rows_of_any_alignment(cuda, M, N, K, left):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("left", [0, 1, 2, 5, 7])
+@pytest.mark.parametrize("K", [1, 7, 9, 15, 17, 127, 455, 2055, 4099, 6185])
+@pytest.mark.parametrize("M", [1, 16, 20, 32, 33])
+def test_few_rows_of_any_alignment(cuda, M, K, left):
+    x, sx, w, sw, b = i8_case(gen(K, cuda), M, 50, K)
+    i8_check(x, sx, w, sw, b, "none", ops.linear_i8(wide_view(x, left, 0), sx, wide_view(w, left + 1, 2), sw, b))
+    _, x, wg, wu, _, _ = gated_bwd_case(gen(K, cuda), M, K, 35)
+    out = ops.gated_linear(wide_view(x, left, 1), wide_view(wg, left, 0), wide_view(wu, left + 1, 2), "silu", save=True)
+    gated_check(x, wg, wu, "silu", out, True)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("left,right", [(0, 8), (8, 8), (3, 0)])
 @pytest.mark.parametrize("M,D", [(5, 96), (3, 4096), (2, 10007)])
@@ -829,7 +841,9 @@ def test_native_refusals():
     """The launchers check by themselves: bad arguments raise before anything is launched."""
     K = ops.feedforward._K
     err = ops.feedforward._C.MccError
-    for call in (lambda: K.gated_forward(1, 8, 8, 9, 0, 8, 0, 0, 8, 0), lambda: K.gated_forward(1, 8, 8, 0, 0, 4, 0, 0, 8, 0),
+    for call in (lambda: K.gated_forward(33, 9, 8, 0, 0, 9, 0, 0, 9, 0, any=True), lambda: K.gated_forward(1, 9, 8, 0, 0, 9, 0, 0, -9, 0, any=True),
+                 lambda: K.linear_i8(33, 1, 9, 0, 0, 9, 0, 0, 9, 0, 0, 0, False, any=True),
+                 lambda: K.gated_forward(1, 8, 8, 9, 0, 8, 0, 0, 8, 0), lambda: K.gated_forward(1, 8, 8, 0, 0, 4, 0, 0, 8, 0),
                  lambda: K.gated_forward(1, 8, 8, 0, 2, 8, 0, 0, 8, 0), lambda: K.gated_forward(1, 0, 8, 0, 0, 8, 0, 0, 8, 0),
                  lambda: K.gated_backward(1, 8, 8, 0, 0, 0, 0, 0, 4, 0, 0, 8, 0, 0, 0),
                  lambda: K.linear_i8(1, 1, 131072, 0, 0, 131072, 0, 0, 131072, 0, 0, 0, False),
