@@ -69,9 +69,8 @@ __device__ __forceinline__ i32x4 load_end(const char* row, int64_t o, int64_t n)
 // NM: matrices on the A side (2: a gate and its projection).  ANY: rows of any
 // address, pitch and length instead of whole aligned pieces: the copy into padded
 // rows would read the weights, write them and read them again (1 x 5500 x 12370
-// int8 39 us, so 26; 32 x
-// 4095 x 8192 gated 75 and 69).  Unaligned loads, which the hardware takes, took 35 and
-// 101.
+// int8 40 us, so 26; 32 x 4095 x 8192 gated 75, so 69).  Unaligned loads, which the
+// hardware takes, took 35 and 101.
 template <class E, int FB, int U, int NW, int NM, bool ANY = false>
 struct FewRows {
   typedef typename E::frag frag;

@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(tile::kThreads, WPE) gated_tile_kernel(GatedPa
   typedef Tile<Bf16, FA, FB, KS, NST, true> T;
   __shared__ __attribute__((aligned(128))) char lds[T::kLds];
   int ta, tb;
-  tile::tile_of(cdiv(p.F, T::RA / 2), cdiv(p.M, T::RB), ta, tb);
+  tile::tile_of((int)blockIdx.x, cdiv(p.F, T::RA / 2), cdiv(p.M, T::RB), ta, tb);
   const int f0 = ta * (T::RA / 2), m0 = tb * T::RB;
   T t;
   t.run(op, lds, f0, m0, 0, (int)((op.kbytes + KS - 1) / KS));

@@ -322,26 +322,74 @@ __global__ void __launch_bounds__(256) gated_dx_rows_kernel(DxRows p) {
   }
 }
 
-// C[b][a] of the tile loop, bf16, or one of gridDim.y partial sums over K in fp32
-template <int FA, int FB, int KS, int NST, int WPE, class TO>
-__global__ void __launch_bounds__(tile::kThreads, WPE) tile_store_kernel(Operands op, TO* out, int steps) {
-  typedef Tile<Bf16, FA, FB, KS, NST, false> T;
-  __shared__ __attribute__((aligned(128))) char lds[T::kLds];
-  int ta, tb;
-  tile::tile_of(cdiv(op.arows, T::RA), cdiv(op.brows, T::RB), ta, tb);
-  const int a0 = ta * T::RA, b0 = tb * T::RB;
-  const int nk = (int)((op.kbytes + KS - 1) / KS);
-  const int k0 = blockIdx.y * steps;
-  T t;
-  t.run(op, lds, a0, b0, k0, min(nk, k0 + steps));
+// Products and sums that one launch does side by side: its workgroups are those
+// of the first product, then of the second, then of the sums.
+struct Product {
+  Operands op;
+  bf16* out;      // C[b][a], or
+  float* part;    // S > 1: S partial sums of it over K
+  int tiles, S, steps;  // K steps a split
+};
+// out = the sum of S partial arrays of n
+struct Sum {
+  const float* part;
+  bf16* out;
+  int64_t n;
+  int S;
+  __host__ __device__ int64_t blocks() const { return (n + 1023) / 1024; }
+};
+struct Work {
+  Product p[2];
+  Sum sum[2];
+  __host__ __device__ int64_t products() const { return (int64_t)p[0].tiles * p[0].S + (int64_t)p[1].tiles * p[1].S; }
+};
 
+// values 1024 i .. of a sum, in order; eight partial arrays in flight (one after the
+// other, 32 of 9 x 640 took 10 us)
+__device__ __forceinline__ void sum_block(const Sum& q, int64_t block) {
+  const int64_t n = q.n, i = (block * 256 + threadIdx.x) * 4;
+  const float* part = q.part;
+  if (i >= n) return;
+  if (n % 4 == 0) {
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    int s = 0;
+    for (; s + 8 <= q.S; s += 8) {
+      f32x4 b[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) b[k] = *reinterpret_cast<const f32x4*>(part + (s + k) * n + i);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] += b[k][e];
+    }
+    for (; s < q.S; ++s) {
+      const f32x4 b = *reinterpret_cast<const f32x4*>(part + s * n + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a[e] += b[e];
+    }
+    *reinterpret_cast<bf16x4*>(q.out + i) = cvt4(a[0], a[1], a[2], a[3]);
+  } else {
+    for (int64_t e = i; e < std::min<int64_t>(i + 4, n); ++e) {
+      float a = 0.f;
+      for (int s = 0; s < q.S; ++s) a += part[s * n + e];
+      q.out[e] = (bf16)a;
+    }
+  }
+}
+__device__ __forceinline__ void sums(const Work& w, int64_t block) {
+  const int64_t n = w.sum[0].blocks();
+  const int k = block >= n;
+  sum_block(w.sum[k], block - k * n);
+}
+__global__ void __launch_bounds__(256) sums_kernel(Work w) { sums(w, blockIdx.x); }
+
+template <int FA, int FB, class TO, class T>
+__device__ __forceinline__ void put_tile(const T& t, char* lds, TO* out, int a0, int b0, const Operands& op) {
   const int wave = threadIdx.x >> 6, wa = wave >> 1, wb = wave & 1;
-  out += (int64_t)blockIdx.y * op.arows * op.brows;
   const bool wide = op.arows % 8 == 0;
   typedef tile::RowStore<TO, FA, FA * FB == 16 && sizeof(TO) == 2> Rows;  // (partial sums are read again at once)
   const Rows rows{lds + wave * Rows::kBytes};
   static_assert(4 * Rows::kBytes <= T::kLds, "row buffers fit the images");
-  __syncthreads();  // every wave has read the last image
 #pragma unroll
   for (int j = 0; j < FB; ++j) {
 #pragma unroll
@@ -355,36 +403,33 @@ __global__ void __launch_bounds__(tile::kThreads, WPE) tile_store_kernel(Operand
   }
 }
 
-// out = the sum of S partial arrays of n, in order; eight of them in flight (one
-// after the other, 32 of 9 x 640 took 10 us)
-__global__ void __launch_bounds__(256) sum_partials_kernel(const float* part, int64_t n, int S, bf16* out) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i >= n) return;
-  if (n % 4 == 0) {
-    f32x4 a = {0.f, 0.f, 0.f, 0.f};
-    int s = 0;
-    for (; s + 8 <= S; s += 8) {
-      f32x4 b[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) b[k] = *reinterpret_cast<const f32x4*>(part + (s + k) * n + i);
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] += b[k][e];
-    }
-    for (; s < S; ++s) {
-      const f32x4 b = *reinterpret_cast<const f32x4*>(part + s * n + i);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) a[e] += b[e];
-    }
-    *reinterpret_cast<bf16x4*>(out + i) = cvt4(a[0], a[1], a[2], a[3]);
-  } else {
-    for (int64_t e = i; e < std::min<int64_t>(i + 4, n); ++e) {
-      float a = 0.f;
-      for (int s = 0; s < S; ++s) a += part[s * n + e];
-      out[e] = (bf16)a;
-    }
+// SUMS: products that are split into partial sums; of the largest tiles all or none
+// are, both ways to store them would not fit the registers
+enum Sums { kNone, kAll, kAny };
+template <int FA, int FB, int KS, int NST, int WPE, Sums SUMS>
+__global__ void __launch_bounds__(tile::kThreads, WPE) products_kernel(Work w) {
+  typedef Tile<Bf16, FA, FB, KS, NST, false> T;
+  __shared__ __attribute__((aligned(128))) char lds[T::kLds];
+  int i = (int)blockIdx.x;
+  const int n0 = w.p[0].tiles * w.p[0].S, n1 = w.p[1].tiles * w.p[1].S;
+  if (i >= n0 + n1) {
+    sums(w, i - n0 - n1);
+    return;
   }
+  const int second = i >= n0;
+  const Product& p = w.p[second];
+  i -= second * n0;
+  const Operands op = p.op;
+  const int split = i / p.tiles;
+  int ta, tb;
+  tile::tile_of(i - split * p.tiles, cdiv(op.arows, T::RA), cdiv(op.brows, T::RB), ta, tb);
+  const int a0 = ta * T::RA, b0 = tb * T::RB;
+  const int nk = (int)((op.kbytes + KS - 1) / KS);
+  T t;
+  t.run(op, lds, a0, b0, split * p.steps, min(nk, (split + 1) * p.steps));
+  __syncthreads();  // every wave has read the last image
+  if (SUMS == kAll || (SUMS == kAny && p.S > 1)) put_tile<FA, FB, float>(t, lds, p.part + (int64_t)split * op.arows * op.brows, a0, b0, op);
+  else put_tile<FA, FB, bf16>(t, lds, p.out, a0, b0, op);
 }
 
 // outputs a workgroup, workgroups a CU, us a step (tile_gemm.h: Form).  640 x
@@ -395,29 +440,64 @@ constexpr tile::Form kForms[] = {{64, 64, 2, 0.27f, 0.5f, 1.2f}, {128, 64, 2, 0.
                                  {128, 128, 2, 0.55f, 1.15f, 2.9f}, {256, 128, 1, 0.86f, 0.86f, 4.8f},
                                  {256, 256, 1, 1.55f, 1.55f, 7.7f}};
 constexpr int kNForms = 5;
-// How a product is done: its form, and into how many sums over K it is split
-// where it has few tiles (1024 x 777 outputs, K = 5472: 37.0 us in 56 tiles of
-// 128 x 128, 15.5 in 4 sums of them and 5 to add these up; 21.8 in 208 tiles of
-// 64 x 64)
+// How the products are done: the form, and into how many sums over K each is split
+// (where it has few tiles: 1024 x 777 outputs, K = 5472, 37.0 us in 56 tiles of 128
+// x 128, 15.5 in 4 sums of them and 5 to add these up; 21.8 in 208 tiles of 64 x 64)
 struct How {
-  int form, S;
+  int form = 0, S[2] = {1, 1};
+  float us = 1e30f;
 };
-How how_of(int64_t arows, int64_t brows, int64_t kbytes) {
-  const int64_t steps = (kbytes + 127) / 128;
-  How best{0, 1};
-  float least = 1e30f;
+struct Shape {
+  int64_t arows, brows, kbytes;
+  int64_t steps() const { return (kbytes + 127) / 128; }
+};
+// a launch of its own, and its tiles' start
+constexpr float kLaunch = 4.f;
+// adding sums up: 8 bytes a value of each
+float join_us(const Shape& x, int S) { return S == 1 ? 0.f : (float)S * x.arows * x.brows * 8.f / 4e6f; }
+// up to 16 sums of at least 4 steps
+constexpr int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16};
+bool splits(const Shape& x, int S) { return S == 1 || x.steps() / S >= 4; }
+
+How how_alone(const Shape& x) {
+  How best;
   for (int f = 0; f < kNForms; ++f) {
-    const int64_t n = tile::workgroups(kForms[f], arows, brows);
-    for (int S = 1; S <= 16 && (S == 1 || steps / S >= 4); ++S) {
-      // adding the sums up: a launch and the pauses of shorter runs, and 8 bytes a value of each
-      const float join = S == 1 ? 0.f : 7.f + (float)S * arows * brows * 8.f / 4e6f;
-      const float us = tile::form_us(kForms[f], n * S, (steps + S - 1) / S) + join;
-      if (us < least) {
-        least = us;
-        best = {f, S};
+    const int64_t n = tile::workgroups(kForms[f], x.arows, x.brows);
+    for (int S : kSplits) {
+      if (!splits(x, S)) break;
+      const float us = tile::form_us(kForms[f], n * S, (x.steps() + S - 1) / S) + join_us(x, S) + (S > 1 ? 7.f : 0.f);
+      if (us < best.us) best = {f, {S, 1}, us};
+    }
+  }
+  best.us += kLaunch;
+  return best;
+}
+// Both products in one launch: none waits for the other's last tiles, and a launch
+// and a join less.  Up to a round of the chip the longest workgroup counts, beyond it
+// their sum and half a workgroup of the ones that end the launch.
+How how_together(const Shape& x, const Shape& y) {
+  How best;
+  for (int f = 0; f < kNForms; ++f) {
+    const tile::Form& t = kForms[f];
+    const int64_t nx = tile::workgroups(t, x.arows, x.brows), ny = tile::workgroups(t, y.arows, y.brows);
+    for (int S : kSplits) {
+      if (!splits(x, S)) break;
+      for (int R : kSplits) {
+        if (!splits(y, R)) break;
+        if (f == kNForms - 1 && (S == 1) != (R == 1)) continue;  // (products_kernel: SUMS)
+        const float lx = (float)((x.steps() + S - 1) / S), ly = (float)((y.steps() + R - 1) / R);
+        const float longest = std::max(lx, ly), shortest = std::min(lx, ly);
+        const int64_t n = nx * S + ny * R, slots = (int64_t)tile::kCus * t.per_cu;
+        float us = longest * (n <= tile::kCus ? t.one : t.full) + t.ends;
+        if (n > slots)
+          us = std::max(us, ((lx * t.full + t.ends) * (float)(nx * S) + (ly * t.full + t.ends) * (float)(ny * R)) / (float)slots +
+                                0.5f * (shortest * t.full + t.ends));
+        us += join_us(x, S) + join_us(y, R) + (S > 1 || R > 1 ? 7.f : 0.f);
+        if (us < best.us) best = {f, {S, R}, us};
       }
     }
   }
+  best.us += kLaunch;
   return best;
 }
 
@@ -434,19 +514,27 @@ int dx_rows_splits(int D, int F) {
 }
 
 struct Plan {
+  int M = 0, D = 0, F = 0;  // of this problem
   int Fp, Mp;
-  How x, w;  // dX and dW
-  int rows;  // K splits of dX by gated_dx_rows_kernel
-  int64_t dgu, dgut, wt, xt, part, total;  // byte offsets
+  Shape sx, sw;       // the products dX and dW
+  How both, x, w;     // together (if that is faster: us), or one after the other
+  int rows;           // K splits of dX by gated_dx_rows_kernel
+  int64_t dgu, dgut, wt, xt, part[2], total;  // byte offsets
 };
-Plan plan_of(int M, int D, int F) {
-  Plan q;
+// (A training loop asks for the same plan again and again, twice a call: the last
+// one is kept, 1.5 us a plan.)
+const Plan& plan_of(int M, int D, int F) {
+  static thread_local Plan q;
+  if (q.M == M && q.D == D && q.F == F) return q;
   // rows of whole 128-byte lines: with rows of 7344 bytes every step's piece of a
   // row lies on two (640 x 17134 x 3672 140 us, of 8192 bytes in proportion 96)
   q.Fp = (int)round_up(F, 64);
   q.Mp = (int)round_up(M, 64);
-  q.x = how_of(D, M, 4 * (int64_t)q.Fp);
-  q.w = how_of(D, 2 * (int64_t)F, 2 * (int64_t)q.Mp);
+  q.sx = {D, M, 4 * (int64_t)q.Fp};
+  q.sw = {D, 2 * (int64_t)F, 2 * (int64_t)q.Mp};
+  q.x = how_alone(q.sx);
+  q.w = how_alone(q.sw);
+  q.both = how_together(q.sx, q.sw);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t o = at;
@@ -458,48 +546,56 @@ Plan plan_of(int M, int D, int F) {
   q.wt = take(2 * (int64_t)D * 2 * q.Fp);
   q.xt = take(2 * (int64_t)D * q.Mp);
   q.rows = M <= 128 ? dx_rows_splits(D, F) : 0;
-  const int64_t pr = 4 * (int64_t)q.rows * M * D;
-  const int64_t px = q.x.S > 1 ? 4 * q.x.S * (int64_t)M * D : 0, pw = q.w.S > 1 ? 4 * q.w.S * 2 * (int64_t)F * D : 0;
-  q.part = take(std::max({px, pw, pr}));
+  const bool both = q.both.us < q.x.us + q.w.us;
+  const int S = both ? q.both.S[0] : q.x.S[0], R = std::max(q.w.S[0], both ? q.both.S[1] : 1);
+  q.part[0] = take(4 * (int64_t)std::max(S > 1 ? S : 0, q.rows) * M * D);
+  q.part[1] = take(R > 1 ? 4 * R * 2 * (int64_t)F * D : 0);
   q.total = at;
+  q.M = M;
+  q.D = D;
+  q.F = F;
   return q;
 }
 
-template <int FA, int FB, int NST, int WPE, class TO>
-void launch_tiles(const Operands& o, TO* out, int steps, int S, hipStream_t s) {
-  const int64_t n = (int64_t)cdiv(o.arows, 64 * FA) * cdiv(o.brows, 64 * FB);
-  MCC_CHECK(launchable(n, tile::kThreads), "gated_linear_bwd: too many rows");
-  const dim3 grid((unsigned)n, (unsigned)S);
-  hipLaunchKernelGGL((tile_store_kernel<FA, FB, 128, NST, WPE, TO>), grid, dim3(tile::kThreads), 0, s, o, out, steps);
-}
-template <class TO> void launch_form(int form, const Operands& o, TO* out, int steps, int S, hipStream_t s) {
-  if (form == 0) launch_tiles<1, 1, 4, 2, TO>(o, out, steps, S, s);
-  else if (form == 1) launch_tiles<2, 1, 3, 2, TO>(o, out, steps, S, s);
-  else if (form == 2) launch_tiles<2, 2, 2, 2, TO>(o, out, steps, S, s);
-  else if (form == 3) launch_tiles<4, 2, 3, 1, TO>(o, out, steps, S, s);
-  else launch_tiles<4, 4, 2, 1, TO>(o, out, steps, S, s);
+// out [brows][arows] = B A^T in the given form and splits
+Product product(const char* a, const char* b, const Shape& x, bf16* out, float* part, int form, int S) {
+  MCC_CHECK(x.kbytes <= (1 << 23), "gated_linear_bwd: row too long");
+  Product p{};
+  p.op.a[0] = p.op.a[1] = a;
+  p.op.b = b;
+  p.op.lda = p.op.ldb = x.kbytes;
+  p.op.arows = (int)x.arows;
+  p.op.brows = (int)x.brows;
+  p.op.kbytes = x.kbytes;
+  p.out = out;
+  p.part = part;
+  const int64_t n = tile::workgroups(kForms[form], x.arows, x.brows);
+  MCC_CHECK(launchable(n * S, tile::kThreads), "gated_linear_bwd: too many rows");
+  p.tiles = (int)n;
+  p.steps = (int)((x.steps() + S - 1) / S);
+  p.S = (int)((x.steps() + p.steps - 1) / p.steps);
+  return p;
 }
 
-// out [brows][arows] = B A^T
-void product(const char* a, int arows, const char* b, int brows, int64_t kbytes, bf16* out, float* part, How how,
-             hipStream_t s) {
-  Operands o;
-  o.a[0] = o.a[1] = a;
-  o.b = b;
-  o.lda = o.ldb = kbytes;
-  o.arows = arows;
-  o.brows = brows;
-  o.kbytes = kbytes;
-  MCC_CHECK(kbytes <= (1 << 23), "gated_linear_bwd: row too long");
-  const int steps = (int)((kbytes + 127) / 128);
-  const int per = cdiv(steps, how.S), S = cdiv(steps, per);
-  if (S == 1) {
-    launch_form<bf16>(how.form, o, out, steps, 1, s);
-  } else {
-    launch_form<float>(how.form, o, part, per, S, s);
-    const int64_t n = (int64_t)arows * brows;
-    hipLaunchKernelGGL(sum_partials_kernel, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, s, part, n, S, out);
-  }
+template <int FA, int FB, int NST, int WPE, Sums SUMS> void launch_tiles(const Work& w, hipStream_t s) {
+  const int64_t n = w.products() + w.sum[0].blocks() + w.sum[1].blocks();
+  MCC_CHECK(launchable(n, tile::kThreads), "gated_linear_bwd: too many rows");
+  hipLaunchKernelGGL((products_kernel<FA, FB, 128, NST, WPE, SUMS>), dim3((unsigned)n), dim3(tile::kThreads), 0, s, w);
+}
+// the products and sums of w, then the sums of partial products
+void run(const Work& w, int form, hipStream_t s) {
+  if (form == 0) launch_tiles<1, 1, 4, 2, kAny>(w, s);
+  else if (form == 1) launch_tiles<2, 1, 3, 2, kAny>(w, s);
+  else if (form == 2) launch_tiles<2, 2, 2, 2, kAny>(w, s);
+  else if (form == 3) launch_tiles<4, 2, 3, 1, kAny>(w, s);
+  else if (w.p[0].S == 1) launch_tiles<4, 4, 2, 1, kNone>(w, s);
+  else launch_tiles<4, 4, 2, 1, kAll>(w, s);
+  Work j{};
+  for (int k = 0; k < 2; ++k)
+    if (w.p[k].S > 1) j.sum[k] = {w.p[k].part, w.p[k].out, (int64_t)w.p[k].op.arows * w.p[k].op.brows, w.p[k].S};
+  const int64_t n = j.sum[0].blocks() + j.sum[1].blocks();
+  MCC_CHECK(launchable(n, 256), "gated_linear_bwd: too many rows");
+  if (n > 0) hipLaunchKernelGGL(sums_kernel, dim3((unsigned)n), dim3(256), 0, s, j);
 }
 
 }  // namespace
@@ -512,13 +608,14 @@ void gated_backward(const GatedBwdParams& p, hipStream_t s) {
   MCC_CHECK(p.ldx >= p.D && p.ldw >= p.D, "gated_linear_bwd: row pitch");
   MCC_CHECK(p.M <= 4000000 && p.F <= (1 << 20), "gated_linear_bwd: too many rows");
   MCC_CHECK(reinterpret_cast<uintptr_t>(p.work) % 256 == 0, "gated_linear_bwd: workspace alignment");
-  const Plan q = plan_of(p.M, p.D, p.F);
+  const Plan& q = plan_of(p.M, p.D, p.F);
   char* w = static_cast<char*>(p.work);
   bf16* dgu = reinterpret_cast<bf16*>(w + q.dgu);
   bf16* dgut = reinterpret_cast<bf16*>(w + q.dgut);
   bf16* wt = reinterpret_cast<bf16*>(w + q.wt);
   bf16* xt = reinterpret_cast<bf16*>(w + q.xt);
-  float* part = reinterpret_cast<float*>(w + q.part);
+  float* part = reinterpret_cast<float*>(w + q.part[0]);
+  float* partw = reinterpret_cast<float*>(w + q.part[1]);
 
   const bool rows = dx_rows_fit(p);
   auto tiles = [](int r, int c) { return cdiv(r, kTP) * cdiv(c, kTP); };
@@ -543,6 +640,14 @@ void gated_backward(const GatedBwdParams& p, hipStream_t s) {
   with_gate(p.act, [&](auto k) {
     hipLaunchKernelGGL((gated_prepare_kernel<decltype(k)::v>), grid, dim3(256), 0, s, t);
   });
+  auto dx = [&](int form, int S) {
+    return product(reinterpret_cast<const char*>(wt), reinterpret_cast<const char*>(dgu), q.sx, static_cast<bf16*>(p.dx), part,
+                   form, S);
+  };
+  auto dw = [&](int form, int S) {
+    return product(reinterpret_cast<const char*>(xt), reinterpret_cast<const char*>(dgut), q.sw, static_cast<bf16*>(p.dw), partw,
+                   form, S);
+  };
   if (rows) {
     const DxRows d{{static_cast<const bf16*>(p.wg), static_cast<const bf16*>(p.wu)}, p.ldw, dgu, p.M, p.D, p.F, q.Fp, part};
     const int S = q.rows;
@@ -551,15 +656,24 @@ void gated_backward(const GatedBwdParams& p, hipStream_t s) {
     else if (p.M <= 32) hipLaunchKernelGGL(gated_dx_rows_kernel<2>, g, dim3(256), 0, s, d);
     else if (p.M <= 64) hipLaunchKernelGGL(gated_dx_rows_kernel<4>, g, dim3(256), 0, s, d);
     else hipLaunchKernelGGL(gated_dx_rows_kernel<8>, g, dim3(256), 0, s, d);
-    const int64_t n = (int64_t)p.M * p.D;
-    hipLaunchKernelGGL(sum_partials_kernel, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, s, part, n, S,
-                       static_cast<bf16*>(p.dx));
+    Work k{};
+    k.sum[0] = {part, static_cast<bf16*>(p.dx), (int64_t)p.M * p.D, S};
+    k.p[0] = dw(q.w.form, q.w.S[0]);
+    run(k, q.w.form, s);
+  } else if (q.both.us < q.x.us + q.w.us) {
+    // the longer workgroups first
+    Work k{};
+    k.p[0] = dx(q.both.form, q.both.S[0]);
+    k.p[1] = dw(q.both.form, q.both.S[1]);
+    if (k.p[0].steps < k.p[1].steps) std::swap(k.p[0], k.p[1]);
+    run(k, q.both.form, s);
   } else {
-    product(reinterpret_cast<const char*>(wt), p.D, reinterpret_cast<const char*>(dgu), p.M, 4 * (int64_t)q.Fp,
-            static_cast<bf16*>(p.dx), part, q.x, s);
+    Work k{};
+    k.p[0] = dx(q.x.form, q.x.S[0]);
+    run(k, q.x.form, s);
+    k.p[0] = dw(q.w.form, q.w.S[0]);
+    run(k, q.w.form, s);
   }
-  product(reinterpret_cast<const char*>(xt), p.D, reinterpret_cast<const char*>(dgut), 2 * p.F, 2 * (int64_t)q.Mp,
-          static_cast<bf16*>(p.dw), part, q.w, s);
   MCC_CHECK(hipGetLastError() == hipSuccess, "gated_linear_bwd: launch failed");
 }
 

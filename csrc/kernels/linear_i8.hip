@@ -39,7 +39,7 @@ __global__ void __launch_bounds__(tile::kThreads, WPE) i8_tile_kernel(LinearI8Pa
   typedef Tile<I8, FA, FB, KS, NST, false> T;
   __shared__ __attribute__((aligned(128))) char lds[T::kLds];
   int ta, tb;
-  tile::tile_of(cdiv(p.N, T::RA), cdiv(p.M, T::RB), ta, tb);
+  tile::tile_of((int)blockIdx.x, cdiv(p.N, T::RA), cdiv(p.M, T::RB), ta, tb);
   const int n0 = ta * T::RA, m0 = tb * T::RB;
   T t;
   t.run(op, lds, n0, m0, 0, (int)((op.kbytes + KS - 1) / KS));

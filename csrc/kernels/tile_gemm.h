@@ -97,8 +97,8 @@ struct Operands {
 // a walk over blocks of 8 B tiles: the 32 CUs of an XCD then hold about 8 x 4
 // tiles and share those 12 operand tiles in their L2.
 template <int G = 8>
-__device__ __forceinline__ void tile_of(int na, int nb, int& ta, int& tb) {
-  const int n = na * nb, i = (int)blockIdx.x;
+__device__ __forceinline__ void tile_of(int i, int na, int nb, int& ta, int& tb) {
+  const int n = na * nb;
   const int q = n >> 3, r = n & 7, x = i & 7;
   const int t = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (i >> 3);
   const int per = G * na;
