@@ -15,6 +15,8 @@
 // the last B row repeat it and are not stored.
 #pragma once
 
+#include <algorithm>
+
 #include "tile_gemm.h"
 
 namespace mcc {
@@ -26,6 +28,17 @@ namespace tile {
 inline float few_rows_us(bool two, int fb, int64_t n) {
   const float us = two ? (fb == 1 ? 0.17f : 0.235f) : (fb == 1 ? 0.145f : 0.19f);
   return us * (n < kCus ? 1.f : (float)n / kCus);
+}
+
+// Groups of 16 (1) or 32 (2) B rows, or tiles (0), which take `tiles` us a step of
+// 128 bytes: what the measured times say; up to 32 rows the weights' way from memory
+// counts, which many workgroups that stream share best
+inline int rows_way(bool two, int64_t a16, int brows, int64_t steps, float tiles) {
+  const int64_t n1 = a16 * ((brows + 15) / 16), n2 = a16 * ((brows + 31) / 32);
+  const float us1 = few_rows_us(two, 1, n1) * (float)steps, us2 = few_rows_us(two, 2, n2) * (float)steps;
+  if (brows <= 16) return 1;
+  if (brows > 32 && (tiles <= std::min(us1, us2) || brows > 16 * 65535)) return 0;
+  return us1 <= us2 ? 1 : 2;
 }
 
 // 16 bytes from any address: the two aligned pieces that hold them (each holds a

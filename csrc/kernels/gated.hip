@@ -143,23 +143,19 @@ void gated_forward(const GatedParams& p, hipStream_t s) {
   MCC_CHECK((p.gate == nullptr) == (p.up == nullptr), "gated_linear: gate and up go together");
   if (p.M == 0) return;
   const Operands o = operands(p);
-  // up to 32 rows the weights' way from memory counts, which many workgroups
-  // that stream share best; above, whatever the measured step times say
-  const int64_t n1 = (int64_t)cdiv(p.F, 16) * cdiv(p.M, 16), n2 = (int64_t)cdiv(p.F, 16) * cdiv(p.M, 32);
   const int64_t steps = (o.kbytes + 127) / 128;
   const int form = tile::best_form(kForms, p.F, p.M, steps);
   const float tiles = tile::form_us(kForms[form], tile::workgroups(kForms[form], p.F, p.M), steps);
-  const float rows1 = tile::few_rows_us(true, 1, n1) * (float)steps;
-  if (p.M <= 16 || (p.M <= 32 ? rows1 <= tile::few_rows_us(true, 2, n2) * (float)steps
-                                   : rows1 < tiles && cdiv(p.M, 16) <= 65535)) {
+  const int way = tile::rows_way(true, cdiv(p.F, 16), p.M, steps, tiles);
+  if (way == 1) {
     const dim3 grid((unsigned)cdiv(p.F, 16), (unsigned)cdiv(p.M, 16));
     const bool eight = o.kbytes >= 4096;
     if (p.any && eight) hipLaunchKernelGGL((gated_rows_kernel<1, 2, 8, true>), grid, dim3(512), 0, s, p, o);
     else if (p.any) hipLaunchKernelGGL((gated_rows_kernel<1, 2, 4, true>), grid, dim3(256), 0, s, p, o);
     else if (eight) hipLaunchKernelGGL((gated_rows_kernel<1, 4, 8, false>), grid, dim3(512), 0, s, p, o);
     else hipLaunchKernelGGL((gated_rows_kernel<1, 4, 4, false>), grid, dim3(256), 0, s, p, o);
-  } else if (p.M <= 32) {
-    const dim3 grid((unsigned)cdiv(p.F, 16));
+  } else if (way == 2) {
+    const dim3 grid((unsigned)cdiv(p.F, 16), (unsigned)cdiv(p.M, 32));
     if (p.any) hipLaunchKernelGGL((gated_rows_kernel<2, 2, 4, true>), grid, dim3(256), 0, s, p, o);
     else hipLaunchKernelGGL((gated_rows_kernel<2, 2, 4, false>), grid, dim3(256), 0, s, p, o);
   } else {

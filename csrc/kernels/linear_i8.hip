@@ -134,23 +134,19 @@ template <class TO> void launch(const LinearI8Params& p, hipStream_t s) {
   o.arows = p.N;
   o.brows = p.M;
   o.kbytes = p.any ? p.K : round_up(p.K, 16);
-  // up to 32 rows the weights' way from memory counts, which many workgroups
-  // that stream share best; above, whatever the measured step times say
-  const int64_t n1 = (int64_t)cdiv(p.N, 16) * cdiv(p.M, 16), n2 = (int64_t)cdiv(p.N, 16) * cdiv(p.M, 32);
   const int64_t steps = (o.kbytes + 127) / 128;
   const int form = tile::best_form(kForms, p.N, p.M, steps);
   const float tiles = tile::form_us(kForms[form], tile::workgroups(kForms[form], p.N, p.M), steps);
-  const float rows1 = tile::few_rows_us(false, 1, n1) * (float)steps;
-  if (p.M <= 16 || (p.M <= 32 ? rows1 <= tile::few_rows_us(false, 2, n2) * (float)steps
-                                   : rows1 < tiles && cdiv(p.M, 16) <= 65535)) {
+  const int way = tile::rows_way(false, cdiv(p.N, 16), p.M, steps, tiles);
+  if (way == 1) {
     const dim3 grid((unsigned)cdiv(p.N, 16), (unsigned)cdiv(p.M, 16));
     const bool eight = o.kbytes >= 4096;
     if (p.any && eight) hipLaunchKernelGGL((i8_rows_kernel<1, 2, 8, true, TO>), grid, dim3(512), 0, s, p, o);
     else if (p.any) hipLaunchKernelGGL((i8_rows_kernel<1, 2, 4, true, TO>), grid, dim3(256), 0, s, p, o);
     else if (eight) hipLaunchKernelGGL((i8_rows_kernel<1, 4, 8, false, TO>), grid, dim3(512), 0, s, p, o);
     else hipLaunchKernelGGL((i8_rows_kernel<1, 4, 4, false, TO>), grid, dim3(256), 0, s, p, o);
-  } else if (p.M <= 32) {
-    const dim3 grid((unsigned)cdiv(p.N, 16));
+  } else if (way == 2) {
+    const dim3 grid((unsigned)cdiv(p.N, 16), (unsigned)cdiv(p.M, 32));
     if (p.any) hipLaunchKernelGGL((i8_rows_kernel<2, 2, 4, true, TO>), grid, dim3(256), 0, s, p, o);
     else hipLaunchKernelGGL((i8_rows_kernel<2, 2, 4, false, TO>), grid, dim3(256), 0, s, p, o);
   } else {

@@ -207,7 +207,7 @@ def gated_linear_bwd(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_
         wg, wu, ldw = wg.contiguous(), wu.contiguous(), D
     _run(dev, _K.gated_backward, M, D, F, kind, dh.data_ptr(), gate.data_ptr(), up.data_ptr(), xa.data_ptr(), ldx,
          wg.data_ptr(), wu.data_ptr(), ldw, dx.data_ptr(), dw.data_ptr(), work.data_ptr())
-    return dx, dw[0], dw[1]
+    return (dx, *dw.unbind())
 
 
 def rmsnorm_i8(x: torch.Tensor, w: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6):
