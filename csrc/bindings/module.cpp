@@ -658,9 +658,9 @@ PYBIND11_MODULE(_C, m) {
   // ---- feed-forward / 8-bit / distillation operators (feedforward.h) ----
   k.def("gated_forward",
         [](int M, int D, int F, int act, uintptr_t x, int64_t ldx, uintptr_t wg, uintptr_t wu, int64_t ldw, uintptr_t h,
-           uintptr_t gate, uintptr_t up, bool any, uintptr_t s) {
+           uintptr_t gate, uintptr_t up, bool any, uintptr_t work, uintptr_t s) {
           gpu::GatedParams p;
-          p.any = any;
+          p.any = any; p.work = ptr<void>(work);
           p.M = M; p.D = D; p.F = F; p.act = act;
           p.x = ptr<void>(x); p.ldx = ldx;
           p.wg = ptr<void>(wg); p.wu = ptr<void>(wu); p.ldw = ldw;
@@ -669,13 +669,18 @@ PYBIND11_MODULE(_C, m) {
         },
         py::arg("M"), py::arg("D"), py::arg("F"), py::arg("act"), py::arg("x"), py::arg("ldx"), py::arg("wg"),
         py::arg("wu"), py::arg("ldw"), py::arg("h"), py::arg("gate") = 0, py::arg("up") = 0, py::arg("any") = false,
-        py::arg("stream") = 0);
+        py::arg("work") = 0, py::arg("stream") = 0);
+  k.def("gated_forward_bytes", &gpu::gated_forward_bytes, py::arg("M"), py::arg("D"), py::arg("F"));
+  k.def("linear_i8_bytes", &gpu::linear_i8_bytes, py::arg("M"), py::arg("N"), py::arg("K"));
   k.attr("ANY_ROWS") = gpu::kAnyRows;
+  k.attr("SPLIT_ROWS") = gpu::kSplitRows;
+  k.attr("SPLIT_BYTES") = gpu::kSplitBytes;
+  k.attr("SPLIT_OUTPUTS") = gpu::kSplitOutputs;
   k.def("linear_i8",
         [](int M, int N, int K, int act, uintptr_t x, int64_t ldx, uintptr_t sx, uintptr_t w, int64_t ldw, uintptr_t sw,
-           uintptr_t bias, uintptr_t y, bool f32, bool any, uintptr_t s) {
+           uintptr_t bias, uintptr_t y, bool f32, bool any, uintptr_t work, uintptr_t s) {
           gpu::LinearI8Params p;
-          p.any = any;
+          p.any = any; p.work = ptr<void>(work);
           p.M = M; p.N = N; p.K = K; p.act = act;
           p.x = ptr<void>(x); p.ldx = ldx; p.sx = ptr<float>(sx);
           p.w = ptr<void>(w); p.ldw = ldw; p.sw = ptr<float>(sw);
@@ -684,7 +689,7 @@ PYBIND11_MODULE(_C, m) {
         },
         py::arg("M"), py::arg("N"), py::arg("K"), py::arg("act"), py::arg("x"), py::arg("ldx"), py::arg("sx"),
         py::arg("w"), py::arg("ldw"), py::arg("sw"), py::arg("bias"), py::arg("y"), py::arg("f32"),
-        py::arg("any") = false, py::arg("stream") = 0);
+        py::arg("any") = false, py::arg("work") = 0, py::arg("stream") = 0);
   // matrices: (src, dst, ld, ldd, rows, cols), pitches and columns in bytes
   k.def("pad_rows",
         [](const std::vector<std::array<int64_t, 6>>& ms, uintptr_t s) {

@@ -33,8 +33,14 @@ struct GatedParams {
   void* gate = nullptr;
   void* up = nullptr;
   bool any = false;  // up to kAnyRows rows of X: rows of any pitch, length and 2-byte alignment
+  void* work = nullptr;  // gated_forward_bytes(M, D, F) bytes (0: none needed), 16-byte aligned
 };
+int64_t gated_forward_bytes(int M, int D, int F);
 constexpr int kAnyRows = 32;
+// Products of more than kSplitRows rows of X with up to kSplitOutputs outputs and rows
+// of kSplitBytes and more may be split over K (gated_forward_bytes, linear_i8_bytes),
+// others never are.
+constexpr int kSplitRows = 16, kSplitBytes = 4096, kSplitOutputs = 1 << 20;
 void gated_forward(const GatedParams& p, hipStream_t s);
 
 // The backward pass of H = f(G) * U from dH [M][F] and the saved G, U [M][F]
@@ -77,7 +83,9 @@ struct LinearI8Params {
   void* y = nullptr;
   bool f32 = false;
   bool any = false;  // up to kAnyRows rows of X: rows of any pitch, length and alignment
+  void* work = nullptr;  // linear_i8_bytes(M, N, K) bytes (0: none needed), 16-byte aligned
 };
+int64_t linear_i8_bytes(int M, int N, int K);
 // the largest K whose sum of products of two int8 cannot pass 32 bits:
 // 131071 * 128 * 128 < 2^31
 constexpr int kLinearI8MaxK = 131071;

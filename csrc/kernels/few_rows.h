@@ -17,6 +17,7 @@
 
 #include <algorithm>
 
+#include "feedforward.h"
 #include "tile_gemm.h"
 
 namespace mcc {
@@ -30,15 +31,41 @@ inline float few_rows_us(bool two, int fb, int64_t n) {
   return us * (n < kCus ? 1.f : (float)n / kCus);
 }
 
-// Groups of 16 (1) or 32 (2) B rows, or tiles (0), which take `tiles` us a step of
-// 128 bytes: what the measured times say; up to 32 rows the weights' way from memory
+// Groups of 16 (1) or 32 (2) B rows, or tiles (0), which take `tiles` us: what the measured times say; up to 32 rows the weights' way from memory
 // counts, which many workgroups that stream share best
-inline int rows_way(bool two, int64_t a16, int brows, int64_t steps, float tiles) {
+// (in us: the time of what is taken)
+inline int rows_way(bool two, int64_t a16, int brows, int64_t steps, float tiles, float& us) {
   const int64_t n1 = a16 * ((brows + 15) / 16), n2 = a16 * ((brows + 31) / 32);
   const float us1 = few_rows_us(two, 1, n1) * (float)steps, us2 = few_rows_us(two, 2, n2) * (float)steps;
+  us = brows <= 16 ? us1 : std::min(us1, us2);
   if (brows <= 16) return 1;
-  if (brows > 32 && (tiles <= std::min(us1, us2) || brows > 16 * 65535)) return 0;
+  if (brows > 32 && (tiles <= us || brows > 16 * 65535)) {
+    us = tiles;
+    return 0;
+  }
   return us1 <= us2 ? 1 : 2;
+}
+
+// Into how many sums over K a product of few tiles (`f`: the smallest) is split, 1:
+// not at all.  `other`: us of the best way without; `bytes`: of an output's partial
+// sum; `weights`: bytes of A, which the step times, taken with operands in the caches,
+// do not hold.  Joining is a launch with its pauses and 2 `bytes` a value of each sum.
+// bf16 152 x 7248 x 1024 with G and U kept, 48 tiles: 41.9 us, in 5 sums 18.7.
+inline int splits_of(const Form& f, int64_t arows, int64_t brows, int64_t steps, int bytes, int64_t weights,
+                     float other) {
+  const int64_t n = workgroups(f, arows, brows);
+  int best = 1;
+  if (brows <= kSplitRows) return best;  // (the waves of few_rows.h split K themselves: 4 x 4288 x 448 11.2 us, in sums 15.2)
+  if (steps * 128 <= kSplitBytes + 128) return best;  // (nothing to gain on a launch; + 128: whatever the rounding of K)
+  for (int S = 2; S <= 16 && n * S <= 2 * kCus && steps / S >= 4; ++S) {
+    const float us = std::max(form_us(f, n * S, (steps + S - 1) / S), (float)weights / 5e6f) + 7.f +
+                     (float)(S * arows * brows * 2 * bytes) / 4e6f;
+    if (us < other) {
+      other = us;
+      best = S;
+    }
+  }
+  return best;
 }
 
 // 16 bytes from any address: the two aligned pieces that hold them (each holds a

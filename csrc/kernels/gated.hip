@@ -86,6 +86,56 @@ __global__ void __launch_bounds__(tile::kThreads, WPE) gated_tile_kernel(GatedPa
   }
 }
 
+// The two projections of one of gridDim.y splits of K: partial sums [split][G | U][M][F]
+template <int FA, int FB, int KS, int NST, int WPE>
+__global__ void __launch_bounds__(tile::kThreads, WPE) gated_part_kernel(GatedParams p, Operands op, int steps) {
+  typedef Tile<Bf16, FA, FB, KS, NST, true> T;
+  __shared__ __attribute__((aligned(128))) char lds[T::kLds];
+  int ta, tb;
+  tile::tile_of((int)blockIdx.x, cdiv(p.F, T::RA / 2), cdiv(p.M, T::RB), ta, tb);
+  const int f0 = ta * (T::RA / 2), m0 = tb * T::RB;
+  const int nk = (int)((op.kbytes + KS - 1) / KS), k0 = (int)blockIdx.y * steps;
+  T t;
+  t.run(op, lds, f0, m0, k0, min(nk, k0 + steps));
+
+  const int wave = threadIdx.x >> 6, wa = wave >> 1, wb = wave & 1;
+  typedef tile::RowStore<float, FA / 2> Rows;
+  const Rows rows{lds + wave * Rows::kBytes};
+  static_assert(4 * Rows::kBytes <= T::kLds, "row buffers fit the images");
+  __syncthreads();  // every wave has read the last image
+  float* out = static_cast<float*>(p.work) + (int64_t)blockIdx.y * 2 * p.M * p.F;
+  float v[16];
+#pragma unroll
+  for (int j = 0; j < FB; ++j) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int i = 0; i < FA / 2; ++i) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = t.acc[k * (FA / 2) + i][j][e];
+        rows.put(i, v);
+      }
+      rows.flush(out + (int64_t)k * p.M * p.F, m0 + T::b_out(wb, j, 0), f0 + T::a_out(wa, 0, 0), p.M, p.F, p.F % 4 == 0);
+    }
+  }
+}
+__global__ void __launch_bounds__(256) gated_join_kernel(GatedParams p, int S) {
+  const int64_t n = (int64_t)p.M * p.F, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const float* part = static_cast<const float*>(p.work) + i;
+  float g = 0.f, u = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < S; ++s) {
+    g += part[2 * s * n];
+    u += part[(2 * s + 1) * n];
+  }
+  with_gate(p.act, [&](auto k) { static_cast<bf16*>(p.h)[i] = (bf16)(gate_f<decltype(k)::v>(g) * u); });
+  if (p.gate) {
+    static_cast<bf16*>(p.gate)[i] = (bf16)g;
+    static_cast<bf16*>(p.up)[i] = (bf16)u;
+  }
+}
+
 template <int FB, int U, int NW, bool ANY>
 __global__ void __launch_bounds__(64 * NW) gated_rows_kernel(GatedParams p, Operands op) {
   typedef FewRows<Bf16, FB, U, NW, 2, ANY> R;
@@ -127,7 +177,26 @@ void launch_tiles(const GatedParams& p, const Operands& o, hipStream_t s) {
   hipLaunchKernelGGL((gated_tile_kernel<FA, FB, 128, NST, WPE, ACT>), grid, dim3(tile::kThreads), 0, s, p, o);
 }
 
+struct Plan {
+  int form, way, S;  // S > 1: the first form, split
+};
+Plan plan_of(int M, int F, int64_t kbytes, bool any) {
+  const int64_t steps = (kbytes + 127) / 128;
+  Plan q;
+  q.form = tile::best_form(kForms, F, M, steps);
+  const float tiles = tile::form_us(kForms[q.form], tile::workgroups(kForms[q.form], F, M), steps);
+  float us;
+  q.way = tile::rows_way(true, cdiv(F, 16), M, steps, tiles, us);
+  q.S = any ? 1 : tile::splits_of(kForms[0], F, M, steps, 8, 2 * F * kbytes, us);
+  return q;
+}
+
 }  // namespace
+
+int64_t gated_forward_bytes(int M, int D, int F) {
+  const int S = plan_of(M, F, round_up(D, 8) * 2, false).S;
+  return S > 1 ? (int64_t)S * 2 * M * F * 4 : 0;
+}
 
 void gated_forward(const GatedParams& p, hipStream_t s) {
   MCC_CHECK(p.M >= 0 && p.D > 0 && p.F > 0, "gated_linear: empty problem");
@@ -143,25 +212,29 @@ void gated_forward(const GatedParams& p, hipStream_t s) {
   MCC_CHECK((p.gate == nullptr) == (p.up == nullptr), "gated_linear: gate and up go together");
   if (p.M == 0) return;
   const Operands o = operands(p);
-  const int64_t steps = (o.kbytes + 127) / 128;
-  const int form = tile::best_form(kForms, p.F, p.M, steps);
-  const float tiles = tile::form_us(kForms[form], tile::workgroups(kForms[form], p.F, p.M), steps);
-  const int way = tile::rows_way(true, cdiv(p.F, 16), p.M, steps, tiles);
-  if (way == 1) {
+  const Plan q = plan_of(p.M, p.F, o.kbytes, p.any);
+  if (q.S > 1) {
+    MCC_CHECK(p.work != nullptr && reinterpret_cast<uintptr_t>(p.work) % 16 == 0, "gated_linear: workspace missing");
+    const int steps = (int)((o.kbytes + 127) / 128), per = cdiv(steps, q.S), S = cdiv(steps, per);
+    const int64_t n = (int64_t)p.M * p.F;  // (at most two workgroups a CU of the first form: a small number)
+    hipLaunchKernelGGL((gated_part_kernel<2, 1, 128, 3, 2>), dim3((unsigned)(cdiv(p.F, 64) * cdiv(p.M, 64)), (unsigned)S),
+                       dim3(tile::kThreads), 0, s, p, o, per);
+    hipLaunchKernelGGL(gated_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p, S);
+  } else if (q.way == 1) {
     const dim3 grid((unsigned)cdiv(p.F, 16), (unsigned)cdiv(p.M, 16));
     const bool eight = o.kbytes >= 4096;
     if (p.any && eight) hipLaunchKernelGGL((gated_rows_kernel<1, 2, 8, true>), grid, dim3(512), 0, s, p, o);
     else if (p.any) hipLaunchKernelGGL((gated_rows_kernel<1, 2, 4, true>), grid, dim3(256), 0, s, p, o);
     else if (eight) hipLaunchKernelGGL((gated_rows_kernel<1, 4, 8, false>), grid, dim3(512), 0, s, p, o);
     else hipLaunchKernelGGL((gated_rows_kernel<1, 4, 4, false>), grid, dim3(256), 0, s, p, o);
-  } else if (way == 2) {
+  } else if (q.way == 2) {
     const dim3 grid((unsigned)cdiv(p.F, 16), (unsigned)cdiv(p.M, 32));
     if (p.any) hipLaunchKernelGGL((gated_rows_kernel<2, 2, 4, true>), grid, dim3(256), 0, s, p, o);
     else hipLaunchKernelGGL((gated_rows_kernel<2, 2, 4, false>), grid, dim3(256), 0, s, p, o);
   } else {
     with_gate(p.act, [&](auto k) {
       constexpr int A = decltype(k)::v;
-      switch (form) {
+      switch (q.form) {
         case 0: launch_tiles<2, 1, 3, 2, A>(p, o, s); break;
         case 1: launch_tiles<2, 2, 2, 2, A>(p, o, s); break;
         case 2: launch_tiles<4, 2, 3, 1, A>(p, o, s); break;

@@ -87,6 +87,50 @@ __global__ void __launch_bounds__(tile::kThreads, WPE) i8_tile_kernel(LinearI8Pa
   }
 }
 
+// One of gridDim.y splits of K: partial sums [split][M][N], 32-bit integers
+template <int FA, int FB, int KS, int NST, int WPE>
+__global__ void __launch_bounds__(tile::kThreads, WPE) i8_part_kernel(LinearI8Params p, Operands op, int steps) {
+  typedef Tile<I8, FA, FB, KS, NST, false> T;
+  __shared__ __attribute__((aligned(128))) char lds[T::kLds];
+  int ta, tb;
+  tile::tile_of((int)blockIdx.x, cdiv(p.N, T::RA), cdiv(p.M, T::RB), ta, tb);
+  const int n0 = ta * T::RA, m0 = tb * T::RB;
+  const int nk = (int)((op.kbytes + KS - 1) / KS), k0 = (int)blockIdx.y * steps;
+  T t;
+  t.run(op, lds, n0, m0, k0, min(nk, k0 + steps));
+
+  const int wave = threadIdx.x >> 6, wa = wave >> 1, wb = wave & 1;
+  typedef tile::RowStore<float, FA> Rows;  // (of the integers' bits)
+  const Rows rows{lds + wave * Rows::kBytes};
+  static_assert(4 * Rows::kBytes <= T::kLds, "row buffers fit the images");
+  __syncthreads();  // every wave has read the last image
+  float* out = static_cast<float*>(p.work) + (int64_t)blockIdx.y * p.M * p.N;
+#pragma unroll
+  for (int j = 0; j < FB; ++j) {
+#pragma unroll
+    for (int i = 0; i < FA; ++i) {
+      float v[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] = __builtin_bit_cast(float, (int)t.acc[i][j][e]);
+      rows.put(i, v);
+    }
+    rows.flush(out, m0 + T::b_out(wb, j, 0), n0 + T::a_out(wa, 0, 0), p.M, p.N, p.N % 4 == 0);
+  }
+}
+template <class TO> __global__ void __launch_bounds__(256) i8_join_kernel(LinearI8Params p, int S) {
+  const int64_t size = (int64_t)p.M * p.N, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= size) return;
+  const int* part = static_cast<const int*>(p.work) + i;
+  int v = 0;
+#pragma unroll 4
+  for (int s = 0; s < S; ++s) v += part[s * size];
+  const int m = (int)(i / p.N), n = (int)(i - (int64_t)m * p.N);
+  const float b = p.bias ? p.bias[n] : 0.f;
+  with_act(p.act, [&](auto k) {
+    static_cast<TO*>(p.y)[i] = (TO)act_i8<decltype(k)::v>((float)v * (p.sx[m] * p.sw[n]) + b);
+  });
+}
+
 template <int FB, int U, int NW, bool ANY, class TO>
 __global__ void __launch_bounds__(64 * NW) i8_rows_kernel(LinearI8Params p, Operands op) {
   typedef FewRows<I8, FB, U, NW, 1, ANY> R;
@@ -125,6 +169,20 @@ void launch_tiles(const LinearI8Params& p, const Operands& o, hipStream_t s) {
 constexpr tile::Form kForms[] = {{64, 64, 2, 0.21f, 0.45f, 0.6f}, {128, 64, 2, 0.28f, 0.69f, 0.8f},
                                  {128, 128, 2, 0.6f, 1.03f, 1.2f}, {256, 256, 1, 1.75f, 1.75f, 4.f}};
 
+struct Plan {
+  int form, way, S;  // S > 1: the first form, split
+};
+Plan plan_of(int M, int N, int64_t kbytes, bool any) {
+  const int64_t steps = (kbytes + 127) / 128;
+  Plan q;
+  q.form = tile::best_form(kForms, N, M, steps);
+  const float tiles = tile::form_us(kForms[q.form], tile::workgroups(kForms[q.form], N, M), steps);
+  float us;
+  q.way = tile::rows_way(false, cdiv(N, 16), M, steps, tiles, us);
+  q.S = any ? 1 : tile::splits_of(kForms[0], N, M, steps, 4, N * kbytes, us);
+  return q;
+}
+
 template <class TO> void launch(const LinearI8Params& p, hipStream_t s) {
   Operands o;
   o.a[0] = o.a[1] = static_cast<const char*>(p.w);
@@ -134,23 +192,27 @@ template <class TO> void launch(const LinearI8Params& p, hipStream_t s) {
   o.arows = p.N;
   o.brows = p.M;
   o.kbytes = p.any ? p.K : round_up(p.K, 16);
-  const int64_t steps = (o.kbytes + 127) / 128;
-  const int form = tile::best_form(kForms, p.N, p.M, steps);
-  const float tiles = tile::form_us(kForms[form], tile::workgroups(kForms[form], p.N, p.M), steps);
-  const int way = tile::rows_way(false, cdiv(p.N, 16), p.M, steps, tiles);
-  if (way == 1) {
+  const Plan q = plan_of(p.M, p.N, o.kbytes, p.any);
+  if (q.S > 1) {
+    MCC_CHECK(p.work != nullptr && reinterpret_cast<uintptr_t>(p.work) % 16 == 0, "linear_i8: workspace missing");
+    const int steps = (int)((o.kbytes + 127) / 128), per = cdiv(steps, q.S), S = cdiv(steps, per);
+    const int64_t n = (int64_t)p.M * p.N;  // (at most two workgroups a CU of the first form: a small number)
+    hipLaunchKernelGGL((i8_part_kernel<1, 1, 128, 4, 2>), dim3((unsigned)(cdiv(p.N, 64) * cdiv(p.M, 64)), (unsigned)S),
+                       dim3(tile::kThreads), 0, s, p, o, per);
+    hipLaunchKernelGGL(i8_join_kernel<TO>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p, S);
+  } else if (q.way == 1) {
     const dim3 grid((unsigned)cdiv(p.N, 16), (unsigned)cdiv(p.M, 16));
     const bool eight = o.kbytes >= 4096;
     if (p.any && eight) hipLaunchKernelGGL((i8_rows_kernel<1, 2, 8, true, TO>), grid, dim3(512), 0, s, p, o);
     else if (p.any) hipLaunchKernelGGL((i8_rows_kernel<1, 2, 4, true, TO>), grid, dim3(256), 0, s, p, o);
     else if (eight) hipLaunchKernelGGL((i8_rows_kernel<1, 4, 8, false, TO>), grid, dim3(512), 0, s, p, o);
     else hipLaunchKernelGGL((i8_rows_kernel<1, 4, 4, false, TO>), grid, dim3(256), 0, s, p, o);
-  } else if (way == 2) {
+  } else if (q.way == 2) {
     const dim3 grid((unsigned)cdiv(p.N, 16), (unsigned)cdiv(p.M, 32));
     if (p.any) hipLaunchKernelGGL((i8_rows_kernel<2, 2, 4, true, TO>), grid, dim3(256), 0, s, p, o);
     else hipLaunchKernelGGL((i8_rows_kernel<2, 2, 4, false, TO>), grid, dim3(256), 0, s, p, o);
   } else {
-    switch (form) {
+    switch (q.form) {
       case 0: launch_tiles<1, 1, 128, 4, 2, TO>(p, o, s); break;
       case 1: launch_tiles<2, 1, 128, 3, 2, TO>(p, o, s); break;
       case 2: launch_tiles<2, 2, 128, 2, 2, TO>(p, o, s); break;
@@ -161,6 +223,11 @@ template <class TO> void launch(const LinearI8Params& p, hipStream_t s) {
 }
 
 }  // namespace
+
+int64_t linear_i8_bytes(int M, int N, int K) {
+  const int S = plan_of(M, N, round_up(K, 16), false).S;
+  return S > 1 ? (int64_t)S * M * N * 4 : 0;
+}
 
 void linear_i8(const LinearI8Params& p, hipStream_t s) {
   MCC_CHECK(p.M >= 0 && p.N > 0 && p.K > 0, "linear_i8: empty problem");

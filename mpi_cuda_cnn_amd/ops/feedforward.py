@@ -23,6 +23,7 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 _GATE = {"none": _K.GATE_NONE, "relu": _K.GATE_RELU, "tanh": _K.GATE_TANH, "silu": _K.GATE_SILU,
          "gelu": _K.GATE_GELU}
+_SPLIT_ROWS, _SPLIT_BYTES, _SPLIT_OUTPUTS = _K.SPLIT_ROWS, _K.SPLIT_BYTES, _K.SPLIT_OUTPUTS
 _ACT = {"none": _K.ACT_NONE, "relu": _K.ACT_RELU, "tanh": _K.ACT_TANH}
 
 
@@ -94,6 +95,10 @@ def _pieces(dev, n, *ts):
     return out
 
 
+def _work(dev, nbytes):
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
 def _run(dev, fn, *args):
     """fn(*args, stream) with dev as the current device (a kernel's launch goes to the current one)."""
     index = dev.index
@@ -131,8 +136,10 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act:
         (xa, ldx), (wg, ldw), (wu, ldu), any_ = _pieces(dev, 8, x, w_gate, w_up)
         if ldu != ldw:  # both weights are read with one pitch
             wg, wu, ldw = wg.contiguous(), wu.contiguous(), wg.shape[1]
+        few = M > _SPLIT_ROWS and 2 * D >= _SPLIT_BYTES and M * F <= _SPLIT_OUTPUTS and not any_  # (others are never split)
+        work = _work(dev, _K.gated_forward_bytes(M, D, F)) if few else None
         _run(dev, _K.gated_forward, M, D, F, kind, xa.data_ptr(), ldx, wg.data_ptr(), wu.data_ptr(), ldw, h.data_ptr(),
-             gate.data_ptr() if save else 0, up.data_ptr() if save else 0, any_)
+             gate.data_ptr() if save else 0, up.data_ptr() if save else 0, any_, work.data_ptr() if work is not None else 0)
     return (h, gate, up) if save else h
 
 
@@ -163,8 +170,11 @@ def linear_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
         (xa, ldx), (wa, ldw), any_ = _pieces(dev, 16, x, w)
         sx, sw = x_scale.contiguous(), w_scale.contiguous()
         bias = b.contiguous() if b is not None else None
+        few = M > _SPLIT_ROWS and K >= _SPLIT_BYTES and M * N <= _SPLIT_OUTPUTS and not any_
+        work = _work(dev, _K.linear_i8_bytes(M, N, K)) if few else None
         _run(dev, _K.linear_i8, M, N, K, _ACT[act], xa.data_ptr(), ldx, sx.data_ptr(), wa.data_ptr(), ldw, sw.data_ptr(),
-             bias.data_ptr() if bias is not None else 0, y.data_ptr(), out_dtype == torch.float32, any_)
+             bias.data_ptr() if bias is not None else 0, y.data_ptr(), out_dtype == torch.float32, any_,
+             work.data_ptr() if work is not None else 0)
     return y
 
 
@@ -276,11 +286,10 @@ def distill_kl(logits: torch.Tensor, t_logits: torch.Tensor, t_index: torch.Tens
         f32 = logits.dtype == torch.float32
         za, ldz = _strided(logits)
         tl, ti = t_logits.contiguous(), t_index.contiguous()
-        nbytes = _K.distill_bytes(M, N, f32)
-        work = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        work = _work(dev, _K.distill_bytes(M, N, f32))
         _run(dev, _K.distill_kl, M, N, K, za.data_ptr(), ldz, f32, tl.data_ptr(), tl.dtype == torch.float32, ti.data_ptr(),
              ti.dtype == torch.int64, temperature, scale, dz.data_ptr() if grad else 0, out == torch.float32,
-             loss.data_ptr(), work.data_ptr() if nbytes else 0)
+             loss.data_ptr(), work.data_ptr() if work is not None else 0)
     return dz, loss
 
 

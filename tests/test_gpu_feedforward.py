@@ -557,6 +557,45 @@ def test_linear_i8_rows_of_any_alignment(cuda, M, N, K, left):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(65, 70, 9000), (152, 1024, 7248), (90, 33, 15608), (300, 129, 4100), (3, 64, 16000),
+                                   (33, 1, 5001), (128, 520, 16383)])
+def test_few_tiles_of_long_rows(cuda, M, N, K):
+    """Products that are split over K: every epilogue."""
+    g = gen(K, cuda)
+    x, sx, w, sw, b = i8_case(g, M, N, K)
+    for act, out in (("none", torch.float32), ("relu", torch.bfloat16), ("tanh", torch.float32)):
+        y = ops.linear_i8(x, sx, w, sw, b, act, out_dtype=out)
+        i8_check(x, sx, w, sw, b, act, y)
+        assert torch.equal(y, ops.linear_i8(x, sx, w, sw, b, act, out_dtype=out))
+    i8_check(x, sx, w, sw, None, "none", ops.linear_i8(x, sx, w, sw))
+    _, x, wg, wu, _, _ = gated_bwd_case(g, M, K, N)
+    for act in ("none", "silu", "gelu", "tanh", "relu"):
+        gated_check(x, wg, wu, act, ops.gated_linear(x, wg, wu, act, save=True), True)
+    gated_check(x, wg, wu, "silu", ops.gated_linear(x, wg, wu, "silu"), False)
+
+
+def test_workspaces():
+    """Split products of few tiles alone ask for a workspace."""
+    K = ops.feedforward._K
+    assert K.gated_forward_bytes(152, 7248, 1024) > 0 and K.linear_i8_bytes(90, 960, 15608) > 0
+    for M, D, F in ((1, 4096, 8192), (777, 1024, 2731), (8192, 4096, 12288), (1, 1, 1), (64, 64, 64)):
+        assert K.gated_forward_bytes(M, D, F) == 0 and K.linear_i8_bytes(M, F, D) == 0
+    # what the wrappers do not ask for is never split
+    for M, F in ((1, 64), (33, 100), (200, 200), (64, 1 << 14), (1024, 1025), (1 << 14, 65), (1, 1 << 20)):
+        for k in (*range(2020, 2048), 100):
+            assert K.gated_forward_bytes(M, k, F) == 0
+        for k in (*range(4070, 4096), 100):
+            assert K.linear_i8_bytes(M, F, k) == 0
+    for M, F in ((16, 64), (1, 5000), (1024, 1025), (1 << 14, 65), (1, (1 << 20) + 1), ((1 << 20) + 1, 1), (300, 3500)):
+        for k in (4097, 20000, 131071):
+            assert K.gated_forward_bytes(M, k, F) == 0 and K.linear_i8_bytes(M, F, k) == 0
+    with pytest.raises(ops.feedforward._C.MccError):
+        K.gated_forward(152, 7248, 1024, 0, 0, 7248, 0, 0, 7248, 0)
+    with pytest.raises(ops.feedforward._C.MccError):
+        K.linear_i8(90, 960, 15616, 0, 0, 15616, 0, 0, 15616, 0, 0, 0, False)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("left", [0, 1, 2, 5, 7])
 @pytest.mark.parametrize("K", [1, 7, 9, 15, 17, 127, 455, 2055, 4099, 6185])
 @pytest.mark.parametrize("M", [1, 16, 20, 32, 33])
