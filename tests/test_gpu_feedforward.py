@@ -210,7 +210,11 @@ GATED_BWD = [(1, 64, 16), (1, 1, 1), (2, 136, 70), (3, 9, 1), (16, 512, 100), (1
              (2078, 70, 1416), (67, 1048, 2845), (1870, 904, 1), (259, 3656, 2888), (2557, 1544, 2694), (8000, 520, 300),
              (8000, 1030, 520), (6000, 2056, 1024), (5550, 4728, 193), (5861, 522, 3385), (4130, 68, 2832),
              (5778, 136, 3466), (5704, 648, 3034), (5921, 646, 2808), (2787, 130, 3160),
-             (7, 4104, 1030), (30, 2056, 1500), (5935, 131, 3777), (9, 640, 2000), (128, 1000, 777), (127, 1001, 777), (129, 1000, 777)]
+             (7, 4104, 1030), (30, 2056, 1500), (5935, 131, 3777), (9, 640, 2000), (128, 1000, 777), (127, 1001, 777), (129, 1000, 777),
+             # the products in one launch or in two, in every form, split and not
+             (4209, 71, 1000), (3490, 329, 324), (1860, 2912, 874), (2249, 1769, 264), (474, 1988, 1488),
+             (229, 3912, 1008), (395, 1488, 2648), (176, 4256, 1848), (368, 3112, 1224), (1189, 533, 5322),
+             (3108, 2256, 219), (2541, 810, 3648), (5236, 2640, 169), (5923, 338, 5417)]
 
 
 @pytest.mark.gpu
