@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(tile::kThreads, WPE) gated_tile_kernel(GatedPa
 
   const int wave = threadIdx.x >> 6, wa = wave >> 1, wb = wave & 1;
   const bool wide = p.F % 8 == 0;
-  typedef tile::RowStore<bf16, FA / 2, FA * FB == 16> Rows;
+  typedef tile::RowStore<bf16, FA / 2, FA * FB >= 12> Rows;
   const Rows rows{lds + wave * Rows::kBytes};
   static_assert(4 * Rows::kBytes <= T::kLds, "row buffers fit the images");
   __syncthreads();  // every wave has read the last image
@@ -164,10 +164,12 @@ __global__ void __launch_bounds__(64 * NW) gated_rows_kernel(GatedParams p, Oper
 // outputs a workgroup (gate and projection at once), workgroups a CU, us a step and
 // for the ends:
 // 1024^3 256 workgroups of the first form 7.8 us, of the second (128) 10.3;
-// 3000 x 512 x 4096 37.0 / 31.3 / 43.9 us; 1024 x 4096 x 4096 84 / 62 / 58 / 79;
-// 4096^3 343 / 251 / 233 / 206
+// 3000 x 512 x 4096 37.0 / 31.3 / 43.9 us; 1024 x 4096 x 4096 84 / 62 / 58 / - / 79;
+// 4096^3 343 / 251 / 233 / - / 206; the fourth is for sizes that leave a last round
+// of the others half empty: 2075 x 4248 x 11904 580 us without it, 435 with
 constexpr tile::Form kForms[] = {{64, 64, 2, 0.27f, 0.67f, 1.6f}, {64, 128, 2, 0.46f, 0.97f, 3.7f},
-                                 {128, 128, 1, 0.9f, 0.9f, 3.9f}, {128, 256, 1, 1.61f, 1.61f, 5.9f}};
+                                 {128, 128, 1, 0.9f, 0.9f, 3.9f}, {128, 192, 1, 1.28f, 1.28f, 4.9f},
+                                 {128, 256, 1, 1.61f, 1.61f, 5.9f}};
 
 template <int FA, int FB, int NST, int WPE, int ACT>
 void launch_tiles(const GatedParams& p, const Operands& o, hipStream_t s) {
@@ -238,6 +240,7 @@ void gated_forward(const GatedParams& p, hipStream_t s) {
         case 0: launch_tiles<2, 1, 3, 2, A>(p, o, s); break;
         case 1: launch_tiles<2, 2, 2, 2, A>(p, o, s); break;
         case 2: launch_tiles<4, 2, 3, 1, A>(p, o, s); break;
+        case 3: launch_tiles<4, 3, 2, 1, A>(p, o, s); break;
         default: launch_tiles<4, 4, 2, 1, A>(p, o, s); break;
       }
     });

@@ -389,7 +389,7 @@ template <int FA, int FB, class TO, class T>
 __device__ __forceinline__ void put_tile(const T& t, char* lds, TO* out, int a0, int b0, const Operands& op) {
   const int wave = threadIdx.x >> 6, wa = wave >> 1, wb = wave & 1;
   const bool wide = op.arows % 8 == 0;
-  typedef tile::RowStore<TO, FA, FA * FB == 16 && sizeof(TO) == 2> Rows;  // (partial sums are read again at once)
+  typedef tile::RowStore<TO, FA, FA * FB >= 12 && sizeof(TO) == 2> Rows;  // (partial sums are read again at once)
   const Rows rows{lds + wave * Rows::kBytes};
   static_assert(4 * Rows::kBytes <= T::kLds, "row buffers fit the images");
 #pragma unroll
@@ -435,13 +435,14 @@ __global__ void __launch_bounds__(tile::kThreads, WPE) products_kernel(Work w) {
 }
 
 // outputs a workgroup, workgroups a CU, us a step (tile_gemm.h: Form).  640 x
-// 16384 x 4096 150 / 126 / 103 / 101 / 92 us; 1024 x 8192 x 8192 216 / 176 / 133 /
-// 113 / 157 us, the last in two sums over K 104; 4096 x 8192 x 64, all ends, 31 / 21
-// / 19 / 25 / 21
+// 16384 x 4096 150 / 126 / 103 / 101 / - / 92 us; 1024 x 8192 x 8192 216 / 176 / 133 /
+// 113 / - / 157 us, the last in two sums over K 104; 4096 x 8192 x 64, all ends, 31 /
+// 21 / 19 / 25 / - / 21; the fifth is for sizes that leave a last round of the others
+// half empty: backward pass of 5578 x 1728 x 2880 270 us without it, 248 with
 constexpr tile::Form kForms[] = {{64, 64, 2, 0.27f, 0.5f, 1.2f}, {128, 64, 2, 0.33f, 0.69f, 1.6f},
                                  {128, 128, 2, 0.55f, 1.15f, 2.9f}, {256, 128, 1, 0.86f, 0.86f, 4.8f},
-                                 {256, 256, 1, 1.55f, 1.55f, 7.7f}};
-constexpr int kNForms = 5;
+                                 {256, 192, 1, 1.24f, 1.24f, 6.2f}, {256, 256, 1, 1.55f, 1.55f, 7.7f}};
+constexpr int kNForms = 6;
 // How the products are done: the form, and into how many sums over K each is split
 // (where it has few tiles: 1024 x 777 outputs, K = 5472, 37.0 us in 56 tiles of 128
 // x 128, 15.5 in 4 sums of them and 5 to add these up; 21.8 in 208 tiles of 64 x 64)
@@ -486,7 +487,7 @@ How how_together(const Shape& x, const Shape& y) {
       if (!splits(x, S)) break;
       for (int R : kSplits) {
         if (!splits(y, R)) break;
-        if (f == kNForms - 1 && (S == 1) != (R == 1)) continue;  // (products_kernel: SUMS)
+        if (f >= kNForms - 2 && (S == 1) != (R == 1)) continue;  // (products_kernel: SUMS)
         const float lx = (float)((x.steps() + S - 1) / S), ly = (float)((y.steps() + R - 1) / R);
         const float longest = std::max(lx, ly), shortest = std::min(lx, ly);
         const int64_t n = nx * S + ny * R, slots = (int64_t)tile::kCus * t.per_cu;
@@ -590,6 +591,8 @@ void run(const Work& w, int form, hipStream_t s) {
   else if (form == 1) launch_tiles<2, 1, 3, 2, kAny>(w, s);
   else if (form == 2) launch_tiles<2, 2, 2, 2, kAny>(w, s);
   else if (form == 3) launch_tiles<4, 2, 3, 1, kAny>(w, s);
+  else if (form == 4 && w.p[0].S == 1) launch_tiles<4, 3, 2, 1, kNone>(w, s);
+  else if (form == 4) launch_tiles<4, 3, 2, 1, kAll>(w, s);
   else if (w.p[0].S == 1) launch_tiles<4, 4, 2, 1, kNone>(w, s);
   else launch_tiles<4, 4, 2, 1, kAll>(w, s);
   Work j{};

@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(tile::kThreads, WPE) i8_tile_kernel(LinearI8Pa
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r32 = lane & 31, g = lane >> 5, wa = wave >> 1, wb = wave & 1;
   const bool wide = p.N % 8 == 0;
-  typedef tile::RowStore<TO, FA, FA * FB == 16> Rows;
+  typedef tile::RowStore<TO, FA, FA * FB >= 12> Rows;
   const Rows rows{lds + wave * Rows::kBytes};
   // the tile's scales and biases, one of each per thread, dealt out through LDS
   float* sw = reinterpret_cast<float*>(lds + 4 * Rows::kBytes);
@@ -162,12 +162,15 @@ void launch_tiles(const LinearI8Params& p, const Operands& o, hipStream_t s) {
     hipLaunchKernelGGL((i8_tile_kernel<FA, FB, KS, NST, WPE, ACT_NONE, TO>), grid, dim3(tile::kThreads), 0, s, p, o);
 }
 
-// outputs a workgroup, workgroups a CU, us a step and for the ends: 640 x 1000 x 4096 9.8 / 11.6 /
-// 16.1 / 37.6 us, 2048^3 16.8 / 15.2 / 13.1 / 25.3, 1024 x 4096 x 4096 29.4 / 25.7
-// / 22.6 / 40.3, 4096^3 117 / 91 / 68 / 60 (and 256 x 128 tiles, which win
-// nowhere, 23.0, 17.7, 29.5, 69)
+// outputs a workgroup, workgroups a CU, us a step and for the ends: 640 x 1000 x 4096
+// 9.8 / 11.6 / 16.1 / - / 37.6 us, 2048^3 16.8 / 15.2 / 13.1 / - / 25.3, 1024 x 4096 x
+// 4096 29.4 / 25.7 / 22.6 / - / 40.3, 4096^3 117 / 91 / 68 / - / 60 (and 256 x 128
+// tiles, which win nowhere, 23.0, 17.7, 29.5, 69); the fourth is for sizes that leave
+// a last round of the others half empty: 3596 x 3944 x 2752 73.9 us without it, 57.8
+// with
 constexpr tile::Form kForms[] = {{64, 64, 2, 0.21f, 0.45f, 0.6f}, {128, 64, 2, 0.28f, 0.69f, 0.8f},
-                                 {128, 128, 2, 0.6f, 1.03f, 1.2f}, {256, 256, 1, 1.75f, 1.75f, 4.f}};
+                                 {128, 128, 2, 0.6f, 1.03f, 1.2f}, {256, 192, 1, 1.4f, 1.4f, 3.5f},
+                                 {256, 256, 1, 1.75f, 1.75f, 4.f}};
 
 struct Plan {
   int form, way, S;  // S > 1: the first form, split
@@ -216,6 +219,7 @@ template <class TO> void launch(const LinearI8Params& p, hipStream_t s) {
       case 0: launch_tiles<1, 1, 128, 4, 2, TO>(p, o, s); break;
       case 1: launch_tiles<2, 1, 128, 3, 2, TO>(p, o, s); break;
       case 2: launch_tiles<2, 2, 128, 2, 2, TO>(p, o, s); break;
+      case 3: launch_tiles<4, 3, 128, 2, 1, TO>(p, o, s); break;
       default: launch_tiles<4, 4, 128, 2, 1, TO>(p, o, s); break;
     }
   }

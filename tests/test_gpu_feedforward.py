@@ -84,7 +84,8 @@ GATED = [(1, 64, 16), (1, 8, 1), (1, 1, 3), (2, 136, 70), (16, 512, 100), (17, 2
          (1000, 520, 130), (4097, 64, 1030), (2050, 136, 4232),
          # the forms that the sizes above do not reach: two groups of 16 rows, 128 x 128 and 128 x 256 tiles
          (24, 72, 4500), (31, 1032, 4099), (1030, 72, 2063), (1024, 200, 2048), (4090, 72, 4090), (4096, 136, 4096),
-         (923, 131, 3336), (909, 67, 3297), (1371, 8, 4804), (62, 2918, 3)]
+         (923, 131, 3336), (909, 67, 3297), (1371, 8, 4804), (62, 2918, 3),
+         (5975, 64, 644), (5970, 136, 645)]
 
 
 @pytest.mark.gpu
@@ -138,7 +139,8 @@ def i8_check(x, sx, w, sw, b, act, y):
 I8 = [(1, 16, 16), (1, 1, 1), (3, 5, 7), (16, 100, 4096), (17, 33, 1000), (33, 64, 144), (64, 1000, 272), (65, 64, 128),
       (128, 128, 640), (130, 70, 130), (640, 1000, 512), (1030, 4100, 176), (4100, 4360, 144), (70, 17, 20000),
       (20, 6000, 500), (32, 4097, 4112), (1500, 1999, 400), (4090, 4090, 272), (4096, 4096, 100), (1870, 1110, 8), (3188, 1322, 8),
-      (3468, 3641, 647)]
+      (3468, 3641, 647),
+      (4364, 2701, 130), (4361, 2704, 272)]
 
 
 @pytest.mark.gpu
@@ -214,7 +216,8 @@ GATED_BWD = [(1, 64, 16), (1, 1, 1), (2, 136, 70), (3, 9, 1), (16, 512, 100), (1
              # the products in one launch or in two, in every form, split and not
              (4209, 71, 1000), (3490, 329, 324), (1860, 2912, 874), (2249, 1769, 264), (474, 1988, 1488),
              (229, 3912, 1008), (395, 1488, 2648), (176, 4256, 1848), (368, 3112, 1224), (1189, 533, 5322),
-             (3108, 2256, 219), (2541, 810, 3648), (5236, 2640, 169), (5923, 338, 5417)]
+             (3108, 2256, 219), (2541, 810, 3648), (5236, 2640, 169), (5923, 338, 5417),
+             (1447, 3976, 832), (4861, 157, 4932), (223, 3984, 1437), (2589, 4016, 120), (68, 856, 5827)]
 
 
 @pytest.mark.gpu
