@@ -548,7 +548,12 @@ const Plan& plan_of(int M, int D, int F) {
   q.dgut = take(2 * 2 * (int64_t)F * q.Mp);
   q.wt = take(2 * (int64_t)D * 2 * q.Fp);
   q.xt = take(2 * (int64_t)D * q.Mp);
-  q.rows = M <= 128 ? dx_rows_splits(D, F) : 0;
+  // dX of few rows from the weights as they are, or transposed beside dG and dU and
+  // then in one launch with dW: one launch less, which short rows are worth (124 x 384 x
+  // 704 17.8 -> 15.8 us)
+  const float weights = 4.f * F * D;  // bytes
+  const float as_they_are = kLaunch + std::max(2.5f, weights / 3.8e6f) + q.w.us, beside = q.both.us + 2.f * weights / 4e6f;
+  q.rows = M <= 128 && as_they_are <= beside ? dx_rows_splits(D, F) : 0;
   const bool both = q.both.us < q.x.us + q.w.us;
   const int S = both ? q.both.S[0] : q.x.S[0], R = std::max(q.w.S[0], both ? q.both.S[1] : 1);
   q.part[0] = take(4 * (int64_t)std::max(S > 1 ? S : 0, q.rows) * M * D);
@@ -622,7 +627,7 @@ void gated_backward(const GatedBwdParams& p, hipStream_t s) {
   float* part = reinterpret_cast<float*>(w + q.part[0]);
   float* partw = reinterpret_cast<float*>(w + q.part[1]);
 
-  const bool rows = dx_rows_fit(p);
+  const bool rows = q.rows > 0 && dx_rows_fit(p);
   auto tiles = [](int r, int c) { return cdiv(r, kTP) * cdiv(c, kTP); };
   Prepare t;
   t.dh = source(p.dh, p.F, p.M, p.F);
