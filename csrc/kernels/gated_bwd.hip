@@ -487,7 +487,7 @@ How how_together(const Shape& x, const Shape& y) {
       if (!splits(x, S)) break;
       for (int R : kSplits) {
         if (!splits(y, R)) break;
-        if (f >= kNForms - 2 && (S == 1) != (R == 1)) continue;  // (products_kernel: SUMS)
+        if (f == kNForms - 1 && (S == 1) != (R == 1)) continue;  // (products_kernel: SUMS)
         const float lx = (float)((x.steps() + S - 1) / S), ly = (float)((y.steps() + R - 1) / R);
         const float longest = std::max(lx, ly), shortest = std::min(lx, ly);
         const int64_t n = nx * S + ny * R, slots = (int64_t)tile::kCus * t.per_cu;
@@ -596,8 +596,7 @@ void run(const Work& w, int form, hipStream_t s) {
   else if (form == 1) launch_tiles<2, 1, 3, 2, kAny>(w, s);
   else if (form == 2) launch_tiles<2, 2, 2, 2, kAny>(w, s);
   else if (form == 3) launch_tiles<4, 2, 3, 1, kAny>(w, s);
-  else if (form == 4 && w.p[0].S == 1) launch_tiles<4, 3, 2, 1, kNone>(w, s);
-  else if (form == 4) launch_tiles<4, 3, 2, 1, kAll>(w, s);
+  else if (form == 4) launch_tiles<4, 3, 2, 1, kAny>(w, s);
   else if (w.p[0].S == 1) launch_tiles<4, 4, 2, 1, kNone>(w, s);
   else launch_tiles<4, 4, 2, 1, kAll>(w, s);
   Work j{};

@@ -217,7 +217,8 @@ GATED_BWD = [(1, 64, 16), (1, 1, 1), (2, 136, 70), (3, 9, 1), (16, 512, 100), (1
              (4209, 71, 1000), (3490, 329, 324), (1860, 2912, 874), (2249, 1769, 264), (474, 1988, 1488),
              (229, 3912, 1008), (395, 1488, 2648), (176, 4256, 1848), (368, 3112, 1224), (1189, 533, 5322),
              (3108, 2256, 219), (2541, 810, 3648), (5236, 2640, 169), (5923, 338, 5417),
-             (1447, 3976, 832), (4861, 157, 4932), (223, 3984, 1437), (2589, 4016, 120), (68, 856, 5827)]
+             (1447, 3976, 832), (4861, 157, 4932), (223, 3984, 1437), (2589, 4016, 120), (68, 856, 5827),
+             (770, 1000, 2700), (777, 1021, 2731), (4723, 1130, 539), (4012, 1328, 4943)]
 
 
 @pytest.mark.gpu
