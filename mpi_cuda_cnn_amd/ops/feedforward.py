@@ -68,17 +68,18 @@ def _pieces(dev, n, *ts):
     where a copy of the weights would cost more than the product."""
     out, todo = [], None
     few = ts[0].shape[0] <= _K.ANY_ROWS
+    kept = []  # the copies' sources: a tensor made here must not go back to the allocator before the kernel is launched
     for t in ts:
         rows, cols = t.shape
         ld, unit = t.stride()
-        if rows <= 1:
-            ld = cols
-        if cols % n == 0 and unit == 1 and cols <= ld < 1 << 22 and ld % n == 0 and t.data_ptr() % 16 == 0:
-            out.append((t, ld))
-            continue
         if unit != 1 and cols > 1:
             t = t.contiguous()
             ld = cols
+        if rows <= 1:
+            ld = cols
+        if cols % n == 0 and cols <= ld < 1 << 22 and ld % n == 0 and t.data_ptr() % 16 == 0:
+            out.append((t, ld))
+            continue
         if few:
             out.append((t, ld))
             todo = ()
@@ -89,6 +90,7 @@ def _pieces(dev, n, *ts):
         if todo is None:
             todo = []
         todo.append((t.data_ptr(), copy.data_ptr(), ld * size, pitch * size, rows, cols * size))
+        kept.append(t)
         out.append((copy, pitch))
     if todo:
         _run(dev, _K.pad_rows, todo)

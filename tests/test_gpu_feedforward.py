@@ -10,6 +10,7 @@ The bounds are worst cases of the arithmetic that the kernels document:
   * an activation in 32 bits by a few units in the last place (2^-20 allowed).
 """
 
+import ctypes
 import math
 
 import pytest
@@ -825,6 +826,69 @@ def test_captured_runs(cuda):
             assert torch.equal(a, b), rep
         for a, b in zip(o2, [*serving(*s_in), *ops.gated_linear_bwd(*rows_in)]):
             assert torch.equal(a, b), rep
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# several operands of one call whose columns are not next to each other
+# ---------------------------------------------------------------------------------------------------------------
+def across(t):
+    """t's values, its columns a row's length apart."""
+    return t.t().contiguous().t()
+
+
+@pytest.mark.parametrize("M,D,F", [(300, 1024, 512), (2048, 512, 1024), (40, 100, 60), (64, 7, 64), (20, 64, 64), (20, 65, 64)])
+def test_copies_of_several_operands(monkeypatch, M, D, F):
+    """What is copied for one call lies in places of its own until the copying kernel has been launched."""
+    ff = ops.feedforward
+    todo = []
+
+    def launch(dev, fn, ms):
+        spans = sorted((a, a + (rows - 1) * pitch + cols) for src, dst, ld, ldd, rows, cols in ms
+                       for a, pitch in ((src, ld), (dst, ldd)))
+        assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:])), spans
+        for src, dst, ld, ldd, rows, cols in ms:
+            ctypes.memset(dst, 0, rows * ldd)
+            for r in range(rows):
+                ctypes.memmove(dst + r * ldd, src + r * ld, cols)
+        todo.extend(ms)
+
+    monkeypatch.setattr(ff, "_run", launch)
+    g = torch.Generator().manual_seed(M)
+    ts = [torch.randn(M, D, generator=g).bfloat16(), *(across(torch.randn(F, D, generator=g).bfloat16()) for _ in range(2))]
+    for x in (ts[0], across(ts[0])):
+        *got, any_ = ff._pieces(torch.device("cpu"), 8, x, ts[1], ts[2])
+        for (t, ld), want in zip(got, ts):
+            assert t.stride() == (ld, 1) and torch.equal(t[:, :D], want) and (any_ or not t[:, D:].any())
+            assert any_ or (ld % 8 == 0 and t.data_ptr() % 16 == 0)
+    assert bool(todo) == (M > 32 and D % 8 != 0)  # (a dense copy of whole pieces is not copied again)
+
+
+ACROSS = [(300, 1024, 512), (2048, 512, 1024), (40, 100, 60), (64, 7, 64), (33, 333, 1000), (20, 64, 64), (20, 65, 64),
+          (152, 7248, 256)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,D,F", ACROSS)
+def test_several_transposed_operands(cuda, M, D, F):
+    g = gen(M + D, cuda)
+    dh, x, wg, wu, gate, up = case = gated_bwd_case(g, M, D, F)
+    for a in (x, across(x)):
+        gated_check(x, wg, wu, "silu", ops.gated_linear(a, across(wg), across(wu), "silu", save=True), True)
+    gated_bwd_check(*case, "silu", ops.gated_linear_bwd(*(across(t) for t in case), "silu"))
+    xq, sx, wq, sw, b = i8_case(g, M, F, D)
+    i8_check(xq, sx, wq, sw, b, "none", ops.linear_i8(across(xq), sx, across(wq), sw, b))
+    # captured: the copies belong to the graph
+    xa, wa, qa = across(x), across(wg), across(xq)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        h = ops.gated_linear(xa, wa, across(wu), "silu")
+        y = ops.linear_i8(qa, sx, across(wq), sw, b)
+    for seed in range(3):
+        xa.copy_(randn(gen(seed, cuda), M, D))
+        graph.replay()
+        gated_check(xa, wg, wu, "silu", h, False)
+        i8_check(xq, sx, wq, sw, b, "none", y)
 
 
 # ---------------------------------------------------------------------------------------------------------------
