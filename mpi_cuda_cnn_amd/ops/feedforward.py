@@ -8,7 +8,8 @@ function of its own.
 
 Rows may be strided views.  The kernels read rows in 16-byte pieces: tensors
 whose rows are not whole pieces, or not aligned to them, are copied into padded
-rows first, in one launch a call; products of up to 32 rows take them as they are.
+rows first, in one launch a call; products of up to 32 rows take them as they are, unless only these rows need a copy and
+the weights are large.
 """
 
 from __future__ import annotations
@@ -62,39 +63,46 @@ def _device(first, *more):
     return first.device
 
 
-def _pieces(dev, n, *ts):
-    """((t or a copy, row pitch), .., any): rows of whole, aligned 16-byte pieces of n elements, zeros behind the last
-    column.  All copies that a call needs are made by one kernel; none for few rows of the first (any is then True),
-    where a copy of the weights would cost more than the product."""
-    out, todo = [], None
-    few = ts[0].shape[0] <= _K.ANY_ROWS
-    kept = []  # the copies' sources: a tensor made here must not go back to the allocator before the kernel is launched
-    for t in ts:
+# Where up to 32 rows alone are not whole pieces they are copied for weights of so many bytes an output column or in all,
+# as the kernel that takes rows of any alignment reads the weights as such rows too (us, with a copy / without):
+# 1 x 4096 x 8192 27.9 / 36.7, 32 x 4096 x 8192 37 / 56, 1 x 4096 x 512 13.0 / 18.2, int8 1 x 16384 x 64 13.6 / 19.5;
+# below it the launch costs more: 1 x 2048 x 2048 12.0 / 10.6, 32 x 512 x 8192 11.8 / 7.9, int8 1 x 8192 x 512 13.0 / 11.0
+_COPY_COLUMN, _COPY_WEIGHTS = 1 << 14, 1 << 25
+
+
+def _pieces(dev, n, x, *weights):
+    """((t or a copy, row pitch) of x and the weights, any): rows of whole, aligned 16-byte pieces of n elements, zeros
+    behind the last column.  All copies that a call needs are made by one kernel; none for few rows of x (any is then
+    True) where a copy would cost more than the product."""
+    ts, part = [], []  # (ts: until the kernel is launched, a tensor made here must not go back to the allocator before)
+    for t in (x, *weights):
         rows, cols = t.shape
         ld, unit = t.stride()
         if unit != 1 and cols > 1:
             t = t.contiguous()
             ld = cols
-        if rows <= 1:
+        elif rows <= 1:
             ld = cols
-        if cols % n == 0 and cols <= ld < 1 << 22 and ld % n == 0 and t.data_ptr() % 16 == 0:
-            out.append((t, ld))
-            continue
-        if few:
-            out.append((t, ld))
-            todo = ()
-            continue
+        if not (cols % n == 0 and cols <= ld < 1 << 22 and ld % n == 0 and t.data_ptr() % 16 == 0):
+            part.append(len(ts))
+        ts.append((t, ld))
+    if part and x.shape[0] <= _K.ANY_ROWS:
+        column = cols * len(weights) * t.element_size()
+        if part != [0] or (column < _COPY_COLUMN and column * rows < _COPY_WEIGHTS):
+            ts.append(True)
+            return ts
+    out, todo = ts[:], []
+    for i in part:
+        t, ld = ts[i]
+        rows, cols = t.shape
         pitch = (cols + n - 1) // n * n
         copy = torch.empty(rows, pitch, dtype=t.dtype, device=dev)
         size = t.element_size()
-        if todo is None:
-            todo = []
         todo.append((t.data_ptr(), copy.data_ptr(), ld * size, pitch * size, rows, cols * size))
-        kept.append(t)
-        out.append((copy, pitch))
+        out[i] = (copy, pitch)
     if todo:
         _run(dev, _K.pad_rows, todo)
-    out.append(todo == ())
+    out.append(False)
     return out
 
 

@@ -863,6 +863,38 @@ def test_copies_of_several_operands(monkeypatch, M, D, F):
     assert bool(todo) == (M > 32 and D % 8 != 0)  # (a dense copy of whole pieces is not copied again)
 
 
+@pytest.mark.parametrize("n,dtype", [(8, torch.bfloat16), (16, torch.int8)])
+@pytest.mark.parametrize("M", [1, 32])
+def test_few_rows_alone_are_copied_for_large_weights(monkeypatch, M, n, dtype):
+    """Large weights of whole pieces are read as such whatever x's alignment."""
+    ff = ops.feedforward
+    todo = []
+    monkeypatch.setattr(ff, "_run", lambda dev, fn, ms: todo.append(ms))
+    size = 16 // n
+    for K, N, copied in ((16384, 64, True), (4096, 1 << 13, True), (1024, 512, False)):
+        K //= size  # (a row of K bytes)
+        x, w = torch.zeros(M, K + 8, dtype=dtype)[:, 1 : K + 1], torch.zeros(N, K, dtype=dtype)
+        todo.clear()
+        (xa, ldx), (wa, ldw), any_ = ff._pieces(torch.device("cpu"), n, x, w)
+        assert wa is w and ldw == K and any_ is not copied
+        assert len(todo) == copied and (not copied or (len(todo[0]) == 1 and todo[0][0][0] == x.data_ptr() and xa is not x))
+        # whole pieces throughout: nothing to do; weights that are not: as they are
+        assert ff._pieces(torch.device("cpu"), n, w[:M], w)[2] is False and len(todo) == copied
+        v = torch.zeros(N, K + 8, dtype=dtype)[:, 1 : K + 1]
+        assert ff._pieces(torch.device("cpu"), n, x, v)[2] is True and len(todo) == copied
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("left", [1, 5])
+@pytest.mark.parametrize("M,D,F", [(1, 4096, 8200), (32, 4096, 4099), (7, 16384, 33), (20, 8192, 70), (17, 512, 100)])
+def test_few_rows_of_another_alignment_than_the_weights(cuda, M, D, F, left):
+    g = gen(M + D, cuda)
+    _, x, wg, wu, _, _ = gated_bwd_case(g, M, D, F)
+    gated_check(x, wg, wu, "silu", ops.gated_linear(wide_view(x, left, 2), wg, wu, "silu", save=True), True)
+    xq, sx, wq, sw, b = i8_case(g, M, F, D)
+    i8_check(xq, sx, wq, sw, b, "none", ops.linear_i8(wide_view(xq, left, 2), sx, wq, sw, b))
+
+
 ACROSS = [(300, 1024, 512), (2048, 512, 1024), (40, 100, 60), (64, 7, 64), (33, 333, 1000), (20, 64, 64), (20, 65, 64),
           (152, 7248, 256)]
 
