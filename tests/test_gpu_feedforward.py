@@ -248,6 +248,24 @@ def test_slopes_are_those_of_the_activations(act):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M", [3, 200])
+def test_tanh_slope_far_from_zero(cuda, M):
+    """dG alone, one value a sum (Wg the identity, Wu zero): its relative error far out, where tanh itself is 1."""
+    n = 64
+    v = torch.linspace(0.1, 40.0, M * n, device=cuda).bfloat16().reshape(M, n)
+    v[:, ::2] *= -1
+    eye, none = torch.eye(n, device=cuda).bfloat16(), torch.zeros(n, n, device=cuda).bfloat16()
+    one = torch.ones(M, n, device=cuda).bfloat16()
+    dx, _, _ = ops.gated_linear_bwd(one, none[:1].expand(M, n), eye, none, v, one, "tanh")
+    ref = 1 / torch.cosh(v.to(D64)) ** 2
+    # the exponent 2 |v| log2(e) of up to 116 has two roundings (its factor's and its own), 2^-23 of ln 2 times it;
+    # exp2, the reciprocal and the products a few units of 2^-24; below 0.7 a tanh off by 5 of them, squared and taken
+    # from 1 to no less than 0.63; two roundings to bf16, dG's and dX's
+    rel = 2.0**-23 * 2 * v.to(D64).abs() + 32 * EPS_F32
+    assert (((dx.to(D64) - ref).abs() / ref) <= rel + 2.02 * EPS_BF16).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("act", ["silu", "gelu", "tanh"])
 def test_gated_gradient_against_differences(cuda, act):
     """The whole backward pass against differences of the forward definition in 64 bits."""
