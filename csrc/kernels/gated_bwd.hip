@@ -609,13 +609,23 @@ void run(const Work& w, int form, hipStream_t s) {
 
 }  // namespace
 
-int64_t gated_backward_bytes(int M, int D, int F) { return plan_of(M, D, F).total; }
+namespace {
+// sizes whose rows of the transposes a buffer load's offset reaches
+void check_sizes(int M, int D, int F) {
+  MCC_CHECK(M > 0 && D > 0 && F > 0, "gated_linear_bwd: empty problem");
+  MCC_CHECK(M <= 4000000 && F <= (1 << 20), "gated_linear_bwd: too many rows");
+}
+}  // namespace
+
+int64_t gated_backward_bytes(int M, int D, int F) {
+  check_sizes(M, D, F);  // (before a workspace of that size is allocated)
+  return plan_of(M, D, F).total;
+}
 
 void gated_backward(const GatedBwdParams& p, hipStream_t s) {
-  MCC_CHECK(p.M > 0 && p.D > 0 && p.F > 0, "gated_linear_bwd: empty problem");
+  check_sizes(p.M, p.D, p.F);
   MCC_CHECK(p.act >= GATE_NONE && p.act <= GATE_GELU, "gated_linear_bwd: unknown activation");
   MCC_CHECK(p.ldx >= p.D && p.ldw >= p.D, "gated_linear_bwd: row pitch");
-  MCC_CHECK(p.M <= 4000000 && p.F <= (1 << 20), "gated_linear_bwd: too many rows");
   MCC_CHECK(reinterpret_cast<uintptr_t>(p.work) % 256 == 0, "gated_linear_bwd: workspace alignment");
   const Plan& q = plan_of(p.M, p.D, p.F);
   char* w = static_cast<char*>(p.work);

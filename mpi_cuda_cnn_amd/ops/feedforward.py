@@ -210,7 +210,8 @@ def _strided(t):
 
 def gated_linear_bwd(dh: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, gate: torch.Tensor,
                      up: torch.Tensor, act: str = "silu"):
-    """(dx [M, D], dw_gate [F, D], dw_up [F, D]), bf16, of gated_linear from dh [M, F] and the (gate, up) that it saved.
+    """(dx [M, D], dw_gate [F, D], dw_up [F, D]), bf16, of gated_linear from dh [M, F] and the (gate, up) that it saved;
+    M <= 4000000, F <= 1048576.
 
     The gradients of the two projections are rounded to bf16, the matrix unit's operand type; sums are fp32 in a fixed
     order (the same call gives the same bits)."""

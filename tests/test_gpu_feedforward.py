@@ -1017,3 +1017,9 @@ def test_native_refusals():
                  lambda: K.distill_kl(1, 200000, 1, 0, 200000, True, 0, True, 0, True, 1.0, 1.0, 0, True, 0, 0)):
         with pytest.raises(err):
             call()
+
+
+@pytest.mark.parametrize("M,D,F", [(4_000_001, 8, 8), (1, 8, (1 << 20) + 1), (0, 8, 8), (8, 0, 8), (8, 8, 0)])
+def test_backward_sizes_are_refused_before_a_workspace_is_made(M, D, F):
+    with pytest.raises(ops.feedforward._C.MccError, match="gated_linear_bwd: (too many rows|empty problem)"):
+        ops.feedforward._K.gated_backward_bytes(M, D, F)
