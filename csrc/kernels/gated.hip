@@ -225,12 +225,14 @@ void gated_forward(const GatedParams& p, hipStream_t s) {
   } else if (q.way == 1) {
     const dim3 grid((unsigned)cdiv(p.F, 16), (unsigned)cdiv(p.M, 16));
     const bool eight = o.kbytes >= 4096;
+    MCC_CHECK(launchable(grid.x, eight ? 512 : 256, grid.y), "gated_linear: too many output columns");
     if (p.any && eight) hipLaunchKernelGGL((gated_rows_kernel<1, 2, 8, true>), grid, dim3(512), 0, s, p, o);
     else if (p.any) hipLaunchKernelGGL((gated_rows_kernel<1, 2, 4, true>), grid, dim3(256), 0, s, p, o);
     else if (eight) hipLaunchKernelGGL((gated_rows_kernel<1, 4, 8, false>), grid, dim3(512), 0, s, p, o);
     else hipLaunchKernelGGL((gated_rows_kernel<1, 4, 4, false>), grid, dim3(256), 0, s, p, o);
   } else if (q.way == 2) {
     const dim3 grid((unsigned)cdiv(p.F, 16), (unsigned)cdiv(p.M, 32));
+    MCC_CHECK(launchable(grid.x, 256, grid.y), "gated_linear: too many output columns");
     if (p.any) hipLaunchKernelGGL((gated_rows_kernel<2, 2, 4, true>), grid, dim3(256), 0, s, p, o);
     else hipLaunchKernelGGL((gated_rows_kernel<2, 2, 4, false>), grid, dim3(256), 0, s, p, o);
   } else {

@@ -206,12 +206,14 @@ template <class TO> void launch(const LinearI8Params& p, hipStream_t s) {
   } else if (q.way == 1) {
     const dim3 grid((unsigned)cdiv(p.N, 16), (unsigned)cdiv(p.M, 16));
     const bool eight = o.kbytes >= 4096;
+    MCC_CHECK(launchable(grid.x, eight ? 512 : 256, grid.y), "linear_i8: too many output columns");
     if (p.any && eight) hipLaunchKernelGGL((i8_rows_kernel<1, 2, 8, true, TO>), grid, dim3(512), 0, s, p, o);
     else if (p.any) hipLaunchKernelGGL((i8_rows_kernel<1, 2, 4, true, TO>), grid, dim3(256), 0, s, p, o);
     else if (eight) hipLaunchKernelGGL((i8_rows_kernel<1, 4, 8, false, TO>), grid, dim3(512), 0, s, p, o);
     else hipLaunchKernelGGL((i8_rows_kernel<1, 4, 4, false, TO>), grid, dim3(256), 0, s, p, o);
   } else if (q.way == 2) {
     const dim3 grid((unsigned)cdiv(p.N, 16), (unsigned)cdiv(p.M, 32));
+    MCC_CHECK(launchable(grid.x, 256, grid.y), "linear_i8: too many output columns");
     if (p.any) hipLaunchKernelGGL((i8_rows_kernel<2, 2, 4, true, TO>), grid, dim3(256), 0, s, p, o);
     else hipLaunchKernelGGL((i8_rows_kernel<2, 2, 4, false, TO>), grid, dim3(256), 0, s, p, o);
   } else {

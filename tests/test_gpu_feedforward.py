@@ -1023,3 +1023,13 @@ def test_native_refusals():
 def test_backward_sizes_are_refused_before_a_workspace_is_made(M, D, F):
     with pytest.raises(ops.feedforward._C.MccError, match="gated_linear_bwd: (too many rows|empty problem)"):
         ops.feedforward._K.gated_backward_bytes(M, D, F)
+
+
+@pytest.mark.parametrize("M", [1, 32])
+@pytest.mark.parametrize("K", [16, 8192])
+def test_more_output_columns_than_a_grid_takes_are_refused(M, K):
+    k, err = ops.feedforward._K, ops.feedforward._C.MccError
+    with pytest.raises(err, match="linear_i8: too many output columns"):
+        k.linear_i8(M, 1 << 30, K, 0, 0, K, 0, 0, K, 0, 0, 0, False)
+    with pytest.raises(err, match="gated_linear: too many output columns"):
+        k.gated_forward(M, K, 1 << 30, 0, 0, K, 0, 0, K, 0)
