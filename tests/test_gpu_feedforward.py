@@ -941,6 +941,64 @@ def test_several_transposed_operands(cuda, M, D, F):
         i8_check(xq, sx, wq, sw, b, "none", y)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_distill_kl_of_long_rows_captured(cuda, dtype):
+    """Rows in chunks, two launches and a workspace: two graphs replayed in turn, with eager calls between; no entries."""
+    sets = [distill_case(gen(s, cuda), 3, n, 9, dtype) for s, n in ((1, 70001), (2, 140000))]
+    for s in sets:
+        ops.distill_kl(*s)
+    torch.cuda.synchronize()
+    graphs, out = [torch.cuda.CUDAGraph() for _ in sets], []
+    for graph, s in zip(graphs, sets):
+        with torch.cuda.graph(graph):
+            out.append(ops.distill_kl(*s, temperature=2.0))
+    for rep in range(3):
+        for s in sets:
+            s[0].copy_(randn(gen(50 + rep, cuda), *s[0].shape, std=2.0, dtype=dtype))
+        for graph in (*graphs, *graphs):
+            graph.replay()
+        for s, (dz, loss) in zip(sets, out):
+            now = ops.distill_kl(*s, temperature=2.0)
+            assert torch.equal(dz, now[0]) and torch.equal(loss, now[1])
+            distill_check(*s, 2.0, 1.0, dz, loss)
+    dz, loss = ops.distill_kl(sets[0][0], sets[0][1][:, :0], sets[0][2][:, :0])
+    assert not dz.any() and not loss.any()
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# whole numbers: sums of -1, 0 and 1 are exact in 32 bits in any order, so that one lost or doubled product shows
+# ---------------------------------------------------------------------------------------------------------------
+def signs(g, *shape):
+    return torch.randint(-1, 2, shape, device=g.device, generator=g).bfloat16()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,D,F", [(1, 4099, 64), (1, 16384, 40), (2, 9000, 17), (16, 2055, 40), (17, 8192, 50), (20, 4104, 70),
+                                   (32, 16385, 35), (33, 5001, 1), (65, 9000, 70), (90, 15608, 33), (128, 16383, 520),
+                                   (152, 7248, 1024), (300, 4100, 129), (777, 1024, 2731), (1030, 2072, 2063),
+                                   (4090, 72, 4090), (2075, 456, 4248), (1000, 8200, 1030), (1371, 8, 4804), (5970, 136, 645)])
+def test_gated_linear_of_whole_numbers(cuda, M, D, F):
+    g = gen(M + D + F, cuda)
+    x, wg, wu = signs(g, M, D), signs(g, F, D), signs(g, F, D)
+    G, U = (x.to(D64) @ w.to(D64).t() for w in (wg, wu))
+    h, gate, up = ops.gated_linear(x, wg, wu, "none", save=True)
+    assert torch.equal(gate, G.bfloat16()) and torch.equal(up, U.bfloat16())
+    assert torch.equal(h, (G.float() * U.float()).bfloat16())  # (one fp32 product of exact factors, rounded once)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,D,F", [*GATED_BWD, (71, 3392, 5760), (1, 4096, 8192), (16, 1024, 9000), (20000, 72, 40), (9000, 264, 520)])
+def test_gated_linear_bwd_of_whole_numbers(cuda, M, D, F):
+    g = gen(M + D + F, cuda)
+    dh, gate, up = (signs(g, M, F) for _ in range(3))
+    x, wg, wu = signs(g, M, D), signs(g, F, D), signs(g, F, D)
+    dG, dU = (dh * up).to(D64), (dh * gate).to(D64)  # (-1, 0 and 1 again)
+    dx, dwg, dwu = ops.gated_linear_bwd(dh, x, wg, wu, gate, up, "none")
+    assert torch.equal(dx, (dG @ wg.to(D64) + dU @ wu.to(D64)).bfloat16())
+    assert torch.equal(dwg, (dG.t() @ x.to(D64)).bfloat16()) and torch.equal(dwu, (dU.t() @ x.to(D64)).bfloat16())
+
+
 # ---------------------------------------------------------------------------------------------------------------
 # refusals (the arguments are looked at before the device: these run without a GPU)
 # ---------------------------------------------------------------------------------------------------------------
