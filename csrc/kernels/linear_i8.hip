@@ -8,8 +8,8 @@
 // output's type.
 //
 // Bound like the bf16 block of gated.hip, at half the bytes and twice the rate: 1 x
-// 8192 x 4096 7.4 us (34 MB at 4.5 TB/s, the launch with it), 640 x 1000 x 4096 9.9,
-// 8192 x 12288 x 4096 330 (2.5 Pop/s).
+// 8192 x 4096 7.4 us (34 MB at 4.5 TB/s, the launch with it), 640 x 1000 x 4096 10.0
+// (operands' way to LDS, 78 KB per us and CU), 8192 x 12288 x 4096 327-355 (2.5 Pop/s).
 #include "feedforward.h"
 #include "few_rows.h"
 #include "gate_act.h"

@@ -8,8 +8,10 @@
 // Statistics are fp32.  max is taken on the bits of |S W|, which order like the
 // values with the infinities and NaN on top, so neither gets lost.
 //
-// Bound by memory: 16384 x 4096 bf16 with a residual 86 us, 470 MB at 5.5 TB/s; one
-// row of 4096 3.4 us, the row's way in, two barriers and the way out.
+// Bound by memory: 16384 x 4096 with a residual, bf16 86-90 us, 470 MB at 5.2 to 5.5
+// TB/s, fp32 155, 872 MB at 5.6; rows that are not whole 16-byte pieces by their single
+// elements (16384 x 4095 bf16 189); one row of 4096 3.2 us, the row's way in, two
+// barriers and the way out.
 #include "feedforward.h"
 #include "mcc/common.h"
 #include "mfma.h"

@@ -26,9 +26,10 @@
 // would read 192 KiB and be bound by LDS.
 //
 // Measured, 256 x 256 tiles over 8192 x 24576 x 4096 for half a second: bf16 1.50
-// PFLOP/s, int8 2.78 Pop/s; a library's bf16 product of that size 1.59.  The matrix
-// unit is busy 85 % of the cycles, and the clock, 1.63 GHz then, gives way to power:
-// with operands of zeros the same loop does 2.1 PFLOP/s and 4.0 Pop/s.
+// PFLOP/s, int8 2.78 Pop/s; a library's bf16 product of that size 1.59.  The clock gives
+// way to power: with operands of zeros the same loop does 2.1 PFLOP/s and 4.0 Pop/s.  The
+// matrix unit is busy 85 % of the cycles at 1.46 to 1.60 GHz in the product dX of
+// gated_bwd.hip at 8192 x 4096 x 24576, whose stores are few.
 //
 // An LDS row of an image is KS bytes = KS/16 slots; slot s of row r holds the
 // row's piece s ^ swz(r), applied on the source address of the load, so that
