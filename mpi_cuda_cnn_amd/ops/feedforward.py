@@ -131,7 +131,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, act:
     """h = act(x @ w_gate.T) * (x @ w_up.T): both projections of a gated feed-forward block, the activation and the
     product in one kernel.
 
-    x [M, D], w_gate, w_up [F, D], bf16; act: none, relu, tanh, silu or gelu (the erf form).  Sums, activation and
+    x [M, D], w_gate, w_up [F, D], bf16, D < 4194304; act: none, relu, tanh, silu or gelu (the erf form).  Sums, activation and
     product are fp32, h [M, F] is rounded once to bf16.  With save=True returns (h, gate, up), the two projections
     rounded to bf16, which gated_linear_bwd takes."""
     kind = _gate_kind(act)

@@ -1091,3 +1091,10 @@ def test_more_output_columns_than_a_grid_takes_are_refused(M, K):
         k.linear_i8(M, 1 << 30, K, 0, 0, K, 0, 0, K, 0, 0, 0, False)
     with pytest.raises(err, match="gated_linear: too many output columns"):
         k.gated_forward(M, K, 1 << 30, 0, 0, K, 0, 0, K, 0)
+
+
+def test_rows_longer_than_a_buffer_offset_takes_are_refused():
+    k, err = ops.feedforward._K, ops.feedforward._C.MccError
+    for M in (1, 33):
+        with pytest.raises(err, match="gated_linear: row pitch too large"):
+            k.gated_forward(M, 1 << 22, 8, 0, 0, 1 << 22, 0, 0, 1 << 22, 0)
